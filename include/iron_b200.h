@@ -412,6 +412,97 @@ int iron_attn_prefill(const uint16_t *q, const uint16_t *k, const uint16_t *v, u
                       const int64_t *kv_strides, const int64_t *out_strides, float scale, int causal,
                       unsigned flags, void *stream);
 
+/* ---- paged KV cache ---------------------------------------------------------------
+ * No reference counterpart: IRON's cache is one padded [kv_heads, max_seq, D] buffer per
+ * sequence, grown by StridedCopy (iron/operators/strided_copy/op.py:18-100). Here keys and
+ * values live in pages of a pool that sequences share:
+ *   k, v     bf16 [layers, num_pages, kv_heads, page_size, head_dim];
+ *   codes    int8 [layers, num_pages, kv_heads, 2, head_dim] and scales fp32 [layers,
+ *            num_pages, kv_heads], or both NULL: the summaries of full pages (below);
+ *   page_table int32 [slots, max_pages]: entry i of a slot holds tokens i * page_size ...,
+ *            -1 for no page;
+ *   lens     int32 [slots]: tokens of each slot;
+ *   refs     int32 [num_pages]: how many table rows hold the page (0: free).
+ * head_dim 64 or 128; page_size 16, 32, 64 or 128; page * max_pages < 2^31; pools and
+ * codes 16-byte aligned. Table entries outside [0, num_pages) are never followed.
+ *
+ * The summary of a full page, per kv head: lo, hi = the smallest and largest key per
+ * dimension, scale = max |key| / 127, codes floor(lo / scale) and ceil(hi / scale) clamped
+ * to [-127, 127]; a page of zeros has scale 0 and codes 0, one with a key that is not
+ * finite scale FLT_MAX and codes -127, 127.
+ */
+typedef struct {
+  uint16_t *k, *v;
+  int8_t *codes;
+  float *scales;
+  int32_t *page_table, *lens, *refs;
+  int layers, slots, num_pages, max_pages, kv_heads, head_dim, page_size;
+} iron_page_pool;
+/* iron_page_append: slot s gets rows index[s, 0], index[s, 1], ... of k_new / v_new (bf16
+ * [layers, slots, num_new, kv_heads, head_dim]), up to the first index outside [0,
+ * num_new), at positions lens[s], lens[s] + 1, ... in every layer; lens_out[s] (may be
+ * lens) gets the new length. Table entries that are still -1 there get the lowest free
+ * pages, in slot order, whose refs become 1; entries that are set are used as they are. A
+ * slot is refused whole (lens_out = lens, nothing written) if the pages run out before it,
+ * if its table row is too short, or if it would write a page that another row holds too;
+ * *status gets the number of refused slots. With codes, pages that become full get their
+ * summary. slots <= 2048. `workspace` >= iron_page_append_workspace_bytes. */
+size_t iron_page_append_workspace_bytes(int slots, int num_pages);
+int iron_page_append(const iron_page_pool *pool, const uint16_t *k_new, const uint16_t *v_new,
+                     const int32_t *index, int num_new, int32_t *lens_out, int32_t *status,
+                     void *workspace, size_t workspace_bytes, unsigned flags, void *stream);
+/* iron_page_fork: slot s becomes what slot source[s] was before the call -- source[s] == s
+ * keeps it, another slot forks (or moves) it, an index outside [0, slots) frees it. Full
+ * pages are shared. A partial last page stays with the old slot itself if that is kept,
+ * else with its lowest new slot; every other one gets the lowest pages that were free
+ * before the call, in slot order, and the valid rows are copied in every layer. Pages past
+ * a slot's length are given back. A slot for which no page is left becomes empty; *status
+ * counts these. page_table_out, lens_out and refs_out get the new state (page_table_out
+ * and refs_out must not overlap the old ones). slots <= 2048. */
+size_t iron_page_fork_workspace_bytes(int slots);
+int iron_page_fork(const iron_page_pool *pool, const int32_t *source, int32_t *page_table_out,
+                   int32_t *lens_out, int32_t *refs_out, int32_t *status, void *workspace,
+                   size_t workspace_bytes, unsigned flags, void *stream);
+/* iron_page_compact: *used = the number of pages with refs > 0; the i-th used page at or
+ * above it moves (all layers, summaries too) to the i-th free page below it, so the used
+ * pages are 0 .. *used - 1 and no more pages move than must. page_table_out and refs_out
+ * (each may be the old one) get the new state. slots <= 2048. */
+size_t iron_page_compact_workspace_bytes(int num_pages);
+int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32_t *refs_out, int32_t *used,
+                      void *workspace, size_t workspace_bytes, unsigned flags, void *stream);
+/* iron_tree_attn: attention of a tree of drafted tokens over one layer of the cache (pool
+ * layers 1; slots = the batch). Node i of sequence b has the parent parents[b, i]: -1 (the
+ * cached prefix itself) or a node j < i; anything else, and every descendant of such a
+ * node, is unused.
+ *   out[b, i, hq] = softmax(scale * q [K_cached; K_path]^T) [V_cached; V_path]
+ * over the lens[b] cached tokens and the nodes on the path to i (i included), fp32
+ * softmax; zeros for an unused node. What the path does not hold has no effect, whatever
+ * its values. q, out bf16 [batch, num_nodes, Hq, D], k_new, v_new bf16 [batch, num_nodes,
+ * kv_heads, D] with element strides {batch, node, head} (3 int64 each, multiples of 8; kv
+ * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024.
+ * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split. */
+size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
+int iron_tree_attn(const iron_page_pool *pool, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
+                   const int32_t *parents, uint16_t *out, int num_nodes, int num_heads, const int64_t *q_strides,
+                   const int64_t *kv_strides, const int64_t *out_strides, float scale, void *workspace,
+                   size_t workspace_bytes, unsigned flags, void *stream);
+/* iron_page_select_attn: decode attention (one query per sequence) over the top_pages pages
+ * of each (sequence, kv head) that a cheap score selects: the last page, the first one,
+ * then by score, the largest first, the lower page on ties. With a = the largest |q| of
+ * the head's query group and q8 = round(q / a * 127), the score of a page is
+ *   float(sum over the group's heads and d of (q8 > 0 ? q8 hi8 : q8 lo8)) * scale
+ * from its summary -- an upper bound of the group's logits up to the rounding of q. The sum
+ * is of integers and the product is one fp32 product, so the selection is the same whatever
+ * the order of summation. (a = 0 or not finite: all q8 = 0.) q, out bf16 [slots, Hq, D]
+ * with element strides {batch, head} (2 int64 each, multiples of 8); selected int32 [slots,
+ * kv_heads, top_pages] gets the pages' places in the slot, ascending, then -1. A slot of
+ * length 0 gives zeros. Hq / kv_heads <= 16. */
+size_t iron_page_select_attn_workspace_bytes(int batch, int num_heads, int kv_heads, int head_dim, int max_pages,
+                                             int top_pages, int page_size);
+int iron_page_select_attn(const iron_page_pool *pool, const uint16_t *q, uint16_t *out, int32_t *selected,
+                          int num_heads, int top_pages, const int64_t *q_strides, const int64_t *out_strides,
+                          float scale, void *workspace, size_t workspace_bytes, unsigned flags, void *stream);
+
 /* ---- tensor-core GEMM (prefill projections) -------------------------------------
  * C = epilogue(A . B^T) on tcgen05 tensor cores with TMEM accumulators: A bf16
  * [M, K] (row pitch lda), B bf16 [N, K] K-major (row pitch ldb), C bf16 [M, N]

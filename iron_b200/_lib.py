@@ -80,12 +80,27 @@ SIGNATURES: dict[str, list] = {
     "iron_attn_decode_qkv_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
     "iron_attn_decode_qkv": [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_float, P,
                              c_size_t, c_uint, P],
+    "iron_page_append_workspace_bytes": [c_int, c_int],
+    "iron_page_append": [P, P, P, P, c_int, P, P, P, c_size_t, c_uint, P],
+    "iron_page_fork_workspace_bytes": [c_int],
+    "iron_page_fork": [P, P, P, P, P, P, P, c_size_t, c_uint, P],
+    "iron_page_compact_workspace_bytes": [c_int],
+    "iron_page_compact": [P, P, P, P, P, c_size_t, c_uint, P],
+    "iron_tree_attn_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "iron_tree_attn": [P, P, P, P, P, P, c_int, c_int, P, P, P, c_float, P, c_size_t, c_uint, P],
+    "iron_page_select_attn_workspace_bytes": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    "iron_page_select_attn": [P, P, P, P, c_int, c_int, P, P, c_float, P, c_size_t, c_uint, P],
     "iron_attn_prefill": [P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P, P, c_float, c_int,
                           c_uint, P],
 }
 _RESTYPES = {"iron_strerror": c_char_p, "iron_attn_decode_workspace_bytes": c_size_t,
              "iron_attn_decode_workspace_bytes_d": c_size_t,
-             "iron_attn_decode_qkv_workspace_bytes": c_size_t}
+             "iron_attn_decode_qkv_workspace_bytes": c_size_t,
+             "iron_page_append_workspace_bytes": c_size_t,
+             "iron_page_fork_workspace_bytes": c_size_t,
+             "iron_page_compact_workspace_bytes": c_size_t,
+             "iron_tree_attn_workspace_bytes": c_size_t,
+             "iron_page_select_attn_workspace_bytes": c_size_t}
 
 class GemvChain(ctypes.Structure):
     """iron_gemv_chain (include/iron_b200.h): the decode-chain extras of
@@ -93,6 +108,15 @@ class GemvChain(ctypes.Structure):
 
     _fields_ = [("residual", c_void_p), ("ss_in", c_void_p), ("eps", c_float), ("ss_out", c_void_p),
                 ("y_weighted", c_void_p), ("weight", c_void_p), ("argmax_keys", c_void_p)]
+
+
+class PagePool(ctypes.Structure):
+    """iron_page_pool (include/iron_b200.h): a paged KV cache (pointers as ints, NULL = none)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("codes", c_void_p), ("scales", c_void_p),
+                ("page_table", c_void_p), ("lens", c_void_p), ("refs", c_void_p), ("layers", c_int),
+                ("slots", c_int), ("num_pages", c_int), ("max_pages", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int), ("page_size", c_int)]
 
 
 _lock = threading.Lock()

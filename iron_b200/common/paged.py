@@ -1,0 +1,106 @@
+"""Base of the operators on a paged KV cache.
+
+IRON's cache is one padded buffer per sequence (iron/applications/llama_3.2_1b/
+llama_npu.py:481-495); pages of a shared pool have no counterpart there. The layout is
+that of ``iron_page_pool`` in include/iron_b200.h:
+
+- ``k_pool``, ``v_pool`` bf16 [layers, pages, kv_heads, page_size, head_dim];
+- ``codes`` int8 [layers, pages, kv_heads, 2, head_dim], ``scales`` fp32 [layers, pages,
+  kv_heads]: the summaries of full pages that PageSelectAttention scores;
+- ``page_table`` int32 [slots, max_pages] (-1: no page), ``lens`` int32 [slots], ``refs``
+  int32 [pages].
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+from .. import _lib
+from .base import MLIROperator
+from .tensor import np_dtype
+
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+class PagedOperator(MLIROperator):
+    """Checks each buffer's device, type, size and order, and keeps one workspace per stream
+    (calls on different streams may overlap; calls on one stream follow one another)."""
+
+    def _check_geometry(self):
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {self.head_dim}")
+        if self.page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {self.page_size}")
+        for name in ("num_pages", "max_pages", "num_kv_heads"):
+            if getattr(self, name) < 1:
+                raise ValueError(f"{name} must be positive, got {getattr(self, name)}")
+        if self.max_pages * self.page_size >= 1 << 31:
+            raise ValueError("max_pages * page_size must be below 2^31 tokens")
+        self._spaces = {}
+        self._wanted = None
+
+    def workspace_bytes(self) -> int:
+        raise NotImplementedError
+
+    def _workspace(self, stream: int):
+        """(address, bytes) of this stream's workspace."""
+        import torch
+
+        ws = self._spaces.get(stream)
+        if ws is None:
+            ws = torch.empty(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
+            self._spaces[stream] = ws
+        return ws.data_ptr(), ws.numel()
+
+    def prepare(self):
+        self._workspace(_lib.current_stream())
+
+    # buffers that may be views with strides (last dimension contiguous)
+    _strided: tuple = ()
+
+    def _check_buffers(self, bufs) -> None:
+        import torch
+
+        if self._wanted is None:
+            kinds = {np.dtype(np.int32): torch.int32, np.dtype(np.int8): torch.int8, np.dtype(np.float32): torch.float32}
+            self._wanted = [(int(np.prod(s.shape, dtype=np.int64)), kinds.get(np.dtype(np_dtype(s.dtype)), torch.bfloat16),
+                             tuple(s.shape), i in self._strided) for i, s in enumerate(self.get_arg_spec())]
+        if len(bufs) != len(self._wanted):
+            raise ValueError(f"{type(self).__name__} takes {len(self._wanted)} buffers, got {len(bufs)}")
+        for i, (t, (numel, dtype, shape, strided)) in enumerate(zip(bufs, self._wanted)):
+            t = getattr(t, "device_tensor", t)
+            if t.dtype is not dtype:
+                raise ValueError(f"buffer {i} of {type(self).__name__} is {t.dtype}, needs {dtype}")
+            if strided and t.shape == shape:
+                if t.stride(-1) != 1:
+                    raise ValueError(f"buffer {i} of {type(self).__name__} needs a contiguous last dimension")
+                continue
+            if t.numel() < numel:
+                raise ValueError(f"buffer {i} of {type(self).__name__} holds {t.numel()} values, needs {numel}")
+            if not t.is_contiguous():
+                raise ValueError(f"buffer {i} of {type(self).__name__} must be contiguous")
+
+    def get_callable(self):
+        _lib.load()
+        written = [i for i, s in enumerate(self.get_arg_spec()) if s.direction != "in"]
+
+        def call(*bufs):
+            self._check_buffers(bufs)
+            self._launch(*bufs, stream=_lib.current_stream())
+            for i in written:
+                if hasattr(bufs[i], "mark_device_written"):
+                    bufs[i].mark_device_written()
+
+        return call
+
+
+def strides(t, shape):
+    """Element strides of the leading dimensions of `t` seen as `shape`."""
+    t = getattr(t, "device_tensor", t)
+    if tuple(t.shape) == tuple(shape):
+        return t.stride()[:-1]
+    out, step = [], 1
+    for n in reversed(shape[1:]):
+        step *= n
+        out.append(step)
+    return tuple(reversed(out))

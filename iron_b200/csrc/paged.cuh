@@ -1,0 +1,186 @@
+// Shared by the operators on a paged KV cache: argument checks and the warp-level
+// attention step on 16 tokens (mma.sync m16n8k16, online softmax in fp32).
+#pragma once
+
+#include "common.cuh"
+
+namespace iron {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The pool's geometry, common to all entry points.
+inline int pool_geometry_check(const iron_page_pool *c) {
+  if (!c || !c->k || !c->v || !c->page_table) return IRON_ERR_NULL;
+  if (c->layers <= 0 || c->slots <= 0 || c->num_pages <= 0 || c->max_pages <= 0 || c->kv_heads <= 0)
+    return IRON_ERR_SHAPE;
+  if (c->layers > 16384 || c->kv_heads > 1024 || c->num_pages > (1 << 24)) return IRON_ERR_SHAPE;
+  if (c->head_dim != 64 && c->head_dim != 128) return IRON_ERR_UNSUPPORTED;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return IRON_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(c->max_pages) * c->page_size > 0x7fffffff) return IRON_ERR_SHAPE;
+  if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->codes)) return IRON_ERR_ALIGN;
+  if ((c->codes != nullptr) != (c->scales != nullptr)) return IRON_ERR_ARG;
+  return IRON_OK;
+}
+
+// ---- a warp's attention over blocks of 16 tokens ------------------------------------------
+// Rows are up to 16 query rows (gid = lane / 4 and gid + 8); tokens come 16 at a time.
+// S = Q K^T takes K fragments straight from the cache rows: the order of k inside an MMA
+// is free as long as Q and K agree, so each lane feeds the 16 contiguous bytes it loaded
+// (k-step ks covers d = 32 (ks / 2) + 8 tid + 4 (ks % 2) + {0, 1 | 2, 3}). V goes through a
+// padded shared tile and ldmatrix.trans.
+
+template <int D>
+struct WarpBlock {
+  uint4 k[2][D / 32];  // K rows gid and gid + 8, 16-byte pieces tid, tid + 4, ...
+  uint4 v[D / 16];     // V pieces i * 32 + lane of the 16 x D tile
+
+  // rows >= n are zero and are not read
+  __device__ __forceinline__ void load(const uint16_t *kp, const uint16_t *vp, int64_t krow, int64_t vrow, int n) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+        k[nt][db] = nt * 8 + gid < n ? ld_act_v4(kp + (nt * 8 + gid) * krow + db * 32 + tid * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int idx = i * 32 + lane, row = idx / (D / 8), c = idx % (D / 8);
+      v[i] = row < n ? ld_act_v4(vp + row * vrow + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+template <int D>
+struct WarpAttn {
+  static constexpr int kVStride = D + 8;  // padded V row: an odd number of 16-byte pieces
+  uint32_t q[D / 16][4];
+  float o[D / 8][4];
+  float m[2], l[2];  // running maximum (log2 units) and this lane's share of the sum, rows gid and gid + 8
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+
+  // q rows at lo and hi (null: a zero row)
+  __device__ __forceinline__ void load_q(const uint16_t *lo, const uint16_t *hi) {
+    const int tid = threadIdx.x & 3;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int d = 32 * (ks >> 1) + 8 * tid + 4 * (ks & 1);
+      const uint2 a = lo ? ld_act_v2(lo + d) : make_uint2(0, 0), b = hi ? ld_act_v2(hi + d) : make_uint2(0, 0);
+      q[ks][0] = a.x;
+      q[ks][1] = b.x;
+      q[ks][2] = a.y;
+      q[ks][3] = b.y;
+    }
+  }
+
+  __device__ __forceinline__ void stage_v(const WarpBlock<D> &x, uint16_t *vs) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int idx = i * 32 + lane, row = idx / (D / 8), c = idx % (D / 8);
+      *reinterpret_cast<uint4 *>(vs + row * kVStride + c * 8) = x.v[i];
+    }
+  }
+
+  // One block whose V tile is staged in vs (stage_v, same warp); bit t of see[0] / see[1]:
+  // row gid / gid + 8 sees token t.
+  __device__ __forceinline__ void step(const uint4 (&k)[2][D / 32], const uint16_t *vs, float scale_log2,
+                                       const uint32_t (&see)[2]) {
+    const int lane = threadIdx.x & 31, tid = lane & 3;
+    float s[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint4 &w = k[nt][ks >> 1];
+        mma_bf16_16816(s[nt], q[ks], (ks & 1) ? w.z : w.x, (ks & 1) ? w.w : w.y);
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = nt * 8 + 2 * tid + (e & 1);
+        s[nt][e] = (see[e >> 1] >> t & 1u) ? s[nt][e] * scale_log2 : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[nt][e]);
+      }
+    float ref[2], al[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      const float mn = fmaxf(m[r], mx[r]);
+      ref[r] = mn == -INFINITY ? 0.f : mn;  // a row that has seen nothing yet
+      al[r] = ex2_approx(m[r] - ref[r]);
+      m[r] = mn;
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[nt][e] = ex2_approx(s[nt][e] - ref[e >> 1]);
+        sum[e >> 1] += s[nt][e];
+      }
+    l[0] = l[0] * al[0] + sum[0];
+    l[1] = l[1] * al[1] + sum[1];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      o[j][0] *= al[0];
+      o[j][1] *= al[0];
+      o[j][2] *= al[1];
+      o[j][3] *= al[1];
+    }
+    // P enters the product with V as two bf16 parts, hi + lo, which hold it to 2^-16: one
+    // bf16 would be off by up to 2^-8 of each term, as much as the output's own rounding.
+    // The second pair of MMAs costs nothing where K and V bound the kernel.
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = s[i >> 1][2 * (i & 1)], p1 = s[i >> 1][2 * (i & 1) + 1];
+      hi[i] = pack_bf16x2(p0, p1);
+      lo[i] = pack_bf16x2(p0 - bf16_lo(hi[i]), p1 - bf16_hi(hi[i]));
+    }
+    __syncwarp();  // V tile stores visible to ldmatrix
+#pragma unroll
+    for (int jp = 0; jp < D / 16; ++jp) {
+      const int row = (lane & 7) + ((lane >> 3) & 1) * 8, col = jp * 16 + (lane >> 4) * 8;
+      const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(vs + row * kVStride + col));
+      uint32_t b[4];
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                   : "r"(addr)
+                   : "memory");
+      mma_bf16_16816(o[2 * jp], hi, b[0], b[1]);
+      mma_bf16_16816(o[2 * jp + 1], hi, b[2], b[3]);
+      mma_bf16_16816(o[2 * jp], lo, b[0], b[1]);
+      mma_bf16_16816(o[2 * jp + 1], lo, b[2], b[3]);
+    }
+    __syncwarp();  // done with the V tile before it is staged again
+  }
+
+  // the row sums over the four lanes of each row
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+  }
+};
+
+// The factor that brings a partial of maximum m (log2 units) to the common maximum M.
+// Partials that saw nothing (m = -inf) get 0, which keeps a NaN in them a NaN.
+__device__ __forceinline__ float rescale(float m, float M) { return exp2f(m - (M == -INFINITY ? 0.f : M)); }
+// O / L; a row that saw nothing is zero.
+__device__ __forceinline__ float normalised(float o, float l) { return l == 0.f ? 0.f : o / l; }
+
+}  // namespace iron

@@ -1,0 +1,378 @@
+// Attention of a tree of drafted tokens over a paged KV cache.
+//
+// Rows: the Hq / Hkv query heads of all nodes share a kv head, so a (sequence, kv head)
+// has num_nodes * group rows that read the same cached K and V. They are cut into groups
+// of 16 rows (the M of mma.sync m16n8k16). Work: every unit = (sequence, kv head, row
+// group) is a list of 64-token tiles -- the cached ones, then the tree's own nodes -- and
+// the concatenation of all units' tiles is cut into as many equal pieces as CTAs fit on
+// the GPU. Lengths are read on the device, so ragged batches and tables wider than the
+// sequences balance all the same. A piece that ends inside a unit leaves its (max, sum,
+// output) as a partial; a second kernel joins them in order.
+#include "paged.cuh"
+
+namespace iron {
+
+constexpr int kTRows = 16;     // rows per unit
+constexpr int kTTile = 64;     // tokens per tile: 16 per warp
+constexpr int kTWarps = 4;
+constexpr int kTMaxBatch = 1024;
+constexpr int kTMaxNodes = 128;
+constexpr int kTCtasPerSm = 4;
+
+struct TreeArgs {
+  const uint16_t *q, *k_new, *v_new, *k, *v;
+  const int *table, *lens, *parents;
+  uint16_t *out;
+  float *ws;  // [CTAs][2][kTRows][2 + D] partial (max, sum, output)
+  int64_t qs[3], ks[3], os[3];  // element strides {batch, node, head}
+  int B, N, Hq, Hkv, groups /* row groups per (sequence, kv head) */, page_shift, M, P;
+  float scale_log2;
+};
+
+// Tiles of a sequence: its cached tokens, then its nodes.
+__device__ __forceinline__ int cached_len(const TreeArgs &a, int b) {
+  return min(max(ld_act_i32(a.lens + b), 0), a.M << a.page_shift);
+}
+
+// Exclusive prefix sum of the sequences' tile counts into pref[0 .. B].
+template <int kThreads>
+__device__ __forceinline__ void tile_prefix(const TreeArgs &a, int *pref, int *warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int nodes = (a.N + kTTile - 1) / kTTile;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    int v = b < a.B ? (cached_len(a, b) + kTTile - 1) / kTTile + nodes : 0;
+    const int mine = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += warp_sums[w];
+      total += warp_sums[w];
+    }
+    if (b < a.B) pref[b] = base + before + v - mine;
+    base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pref[a.B] = base;
+  __syncthreads();
+}
+
+// Piece c of `total` tiles over `ctas` pieces starts here.
+__device__ __forceinline__ int64_t piece_start(int64_t total, int c, int ctas) { return total * c / ctas; }
+// The piece that holds tile w.
+__device__ __forceinline__ int piece_of(int64_t total, int64_t w, int ctas) {
+  return static_cast<int>(((w + 1) * ctas - 1) / total);
+}
+
+// Node i's path as bits (128), or none and `used` false. parents in shared memory.
+__device__ __forceinline__ bool tree_path(const int *parents, int i, uint32_t (&bits)[kTMaxNodes / 32]) {
+#pragma unroll
+  for (int w = 0; w < kTMaxNodes / 32; ++w) bits[w] = 0;
+  int j = i;
+  while (true) {
+#pragma unroll
+    for (int w = 0; w < kTMaxNodes / 32; ++w)
+      if (j >> 5 == w) bits[w] |= 1u << (j & 31);
+    const int p = parents[j];
+    if (p == -1) return true;
+    if (p < 0 || p >= j) break;
+    j = p;
+  }
+#pragma unroll
+  for (int w = 0; w < kTMaxNodes / 32; ++w) bits[w] = 0;
+  return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(TreeArgs a) {
+  using Attn = WarpAttn<D>;
+  constexpr int kVBytes = kTWarps * 16 * Attn::kVStride * 2;
+  constexpr int kOBytes = kTWarps * kTRows * D * 4;
+  __shared__ __align__(16) uint8_t smem[kVBytes > kOBytes ? kVBytes : kOBytes];  // V tiles, then the merge
+  __shared__ float red_m[kTWarps][kTRows], red_l[kTWarps][kTRows];
+  __shared__ int pref[kTMaxBatch + 1], warp_sums[kTWarps];
+  __shared__ int parents[kTMaxNodes];
+  __shared__ uint32_t paths[kTRows][kTMaxNodes / 32];
+  __shared__ uint32_t usable[kTMaxNodes / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
+  uint16_t *vs = reinterpret_cast<uint16_t *>(smem) + warp * 16 * Attn::kVStride;
+  float (*red_o)[kTRows][D] = reinterpret_cast<float (*)[kTRows][D]>(smem);
+  pdl_launch_dependents();
+  pdl_wait();
+  tile_prefix<32 * kTWarps>(a, pref, warp_sums);
+  const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
+  const int64_t total = static_cast<int64_t>(pref[a.B]) * per;
+  const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));  // none is empty
+  if (static_cast<int>(blockIdx.x) >= pieces) return;
+  int64_t w = piece_start(total, blockIdx.x, pieces);
+  const int64_t w_end = piece_start(total, blockIdx.x + 1, pieces);
+  const int page = 1 << a.page_shift;
+
+  while (w < w_end) {
+    // the unit that holds tile w: the last sequence that starts at or before it
+    const int x = static_cast<int>(w / per);
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    const int b = lo, tiles = pref[b + 1] - pref[b];
+    const int64_t rem = w - static_cast<int64_t>(pref[b]) * per;
+    const int unit = static_cast<int>(rem / tiles), first = static_cast<int>(rem % tiles);
+    const int count = static_cast<int>(min(static_cast<int64_t>(tiles - first), w_end - w));
+    const int h = unit / a.groups, row0 = unit % a.groups * kTRows;
+    const int len = cached_len(a, b), ctiles = (len + kTTile - 1) / kTTile;
+    const int *table = a.table + static_cast<int64_t>(b) * a.M;
+
+    Attn at;
+    at.clear();
+    const int r_lo = row0 + gid, r_hi = row0 + gid + 8, rows = a.N * g;
+    const uint16_t *qb = a.q + b * a.qs[0];
+    at.load_q(r_lo < rows ? qb + r_lo / g * a.qs[1] + (h * g + r_lo % g) * a.qs[2] : nullptr,
+              r_hi < rows ? qb + r_hi / g * a.qs[1] + (h * g + r_hi % g) * a.qs[2] : nullptr);
+    if (first + count > ctiles) {  // the tree's nodes are part of this piece: their paths
+      for (int i = threadIdx.x; i < kTMaxNodes; i += 32 * kTWarps)
+        parents[i] = i < a.N ? ld_act_i32(a.parents + static_cast<int64_t>(b) * a.N + i) : -2;
+      __syncthreads();
+      if (threadIdx.x < kTMaxNodes) {
+        uint32_t bits[kTMaxNodes / 32];
+        const int i = threadIdx.x;
+        const bool used = i < a.N && tree_path(parents, i, bits);
+        const unsigned all = __ballot_sync(0xffffffffu, used);
+        if (lane == 0) usable[warp] = all;
+      }
+      if (threadIdx.x < kTRows) {
+        uint32_t bits[kTMaxNodes / 32] = {};
+        const int i = (row0 + threadIdx.x) / g;
+        if (i < a.N) tree_path(parents, i, bits);
+#pragma unroll
+        for (int q = 0; q < kTMaxNodes / 32; ++q) paths[threadIdx.x][q] = bits[q];
+      }
+      __syncthreads();
+    }
+    WarpBlock<D> blk;
+    for (int i = first; i < first + count; ++i) {
+      uint32_t see[2];
+      if (i < ctiles) {
+        const int t = i * kTTile + warp * 16, n = min(16, len - t);
+        if (n <= 0) continue;
+        const int p = ld_act_i32(table + (t >> a.page_shift));
+        const bool ok = p >= 0 && p < a.P;
+        const int64_t at0 = ((static_cast<int64_t>(ok ? p : 0) * a.Hkv + h) << a.page_shift) + (t & (page - 1));
+        blk.load(a.k + at0 * D, a.v + at0 * D, D, D, ok ? n : 0);
+        see[0] = see[1] = ok ? 0xffffu >> (16 - n) : 0u;
+      } else {
+        const int j0 = (i - ctiles) * kTTile + warp * 16;
+        if (j0 >= a.N) continue;
+        const uint32_t can = usable[j0 >> 5] >> (j0 & 31) & 0xffffu;
+        const int64_t at0 = b * a.ks[0] + j0 * a.ks[1] + h * a.ks[2];
+        // unused nodes are not read: rows past the last usable one by n, others by the mask
+        blk.load(a.k_new + at0, a.v_new + at0, a.ks[1], a.ks[1], can ? 32 - __clz(can) : 0);
+        see[0] = paths[gid][j0 >> 5] >> (j0 & 31) & 0xffffu;
+        see[1] = paths[gid + 8][j0 >> 5] >> (j0 & 31) & 0xffffu;
+        // a masked token's probability is 0, but 0 * inf is not: values that are not finite
+        // leave the tile and are added to the rows that see them
+        bool odd = false;
+#pragma unroll
+        for (int v = 0; v < D / 16; ++v) {
+          uint32_t *e = reinterpret_cast<uint32_t *>(&blk.v[v]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if ((e[c] & 0x7f80u) == 0x7f80u) e[c] &= 0xffff0000u, odd = true;
+            if ((e[c] & 0x7f800000u) == 0x7f800000u) e[c] &= 0xffffu, odd = true;
+          }
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+          for (int t = 0; t < 16; ++t) {
+            if (!(can >> t & 1u)) continue;
+            const uint16_t *vt = a.v_new + at0 + t * a.ks[1];
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float f = bf16_bits_to_float(ld_act_u16(vt + 8 * j + 2 * tid + e));
+                if (isfinite(f)) continue;
+                if (see[0] >> t & 1u) at.o[j][e] += f;
+                if (see[1] >> t & 1u) at.o[j][2 + e] += f;
+              }
+          }
+        }
+      }
+      at.stage_v(blk, vs);
+      at.step(blk.k, vs, a.scale_log2, see);
+    }
+    at.finish();
+    __syncthreads();  // every warp is done with the V tiles
+    if (tid == 0) {
+      red_m[warp][gid] = at.m[0];
+      red_m[warp][gid + 8] = at.m[1];
+      red_l[warp][gid] = at.l[0];
+      red_l[warp][gid + 8] = at.l[1];
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      *reinterpret_cast<float2 *>(&red_o[warp][gid][8 * j + 2 * tid]) = make_float2(at.o[j][0], at.o[j][1]);
+      *reinterpret_cast<float2 *>(&red_o[warp][gid + 8][8 * j + 2 * tid]) = make_float2(at.o[j][2], at.o[j][3]);
+    }
+    __syncthreads();
+    const bool whole = count == tiles;
+    const bool has_tree = first + count > ctiles;
+    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * kTRows * (2 + D);
+    for (int idx = threadIdx.x; idx < kTRows * D; idx += 32 * kTWarps) {
+      const int r = idx / D, d = idx % D;
+      float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int q = 0; q < kTWarps; ++q) M = fmaxf(M, red_m[q][r]);
+#pragma unroll
+      for (int q = 0; q < kTWarps; ++q) {
+        const float f = rescale(red_m[q][r], M);
+        L += red_l[q][r] * f;
+        O += red_o[q][r][d] * f;
+      }
+      // an unused node: its path is empty (a used one holds the node itself)
+      bool dead = false;
+      if (has_tree) dead = (paths[r][0] | paths[r][1] | paths[r][2] | paths[r][3]) == 0;
+      if (whole) {
+        const int rr = row0 + r;
+        if (rr < rows)
+          a.out[b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d] =
+              float_to_bf16_bits(dead ? 0.f : normalised(O, L));
+      } else {
+        if (d == 0) {
+          part[r * (2 + D)] = M;
+          part[r * (2 + D) + 1] = dead ? -1.f : L;  // -1: the join writes zeros
+        }
+        part[r * (2 + D) + 2 + d] = O;
+      }
+    }
+    __syncthreads();  // shared memory is used again
+    w += count;
+  }
+}
+
+// Joins the partials of one unit, in the order of its tiles. Units that one piece held
+// whole have nothing to join.
+template <int D>
+__global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a, int ctas) {
+  __shared__ int sums[4];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
+  const int b = blockIdx.x / per, unit = blockIdx.x % per;
+  const int nodes = (a.N + kTTile - 1) / kTTile;
+  // tiles before this sequence and in all
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < a.B; i += 128) {
+    const int t = (cached_len(a, i) + kTTile - 1) / kTTile + nodes;
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  __shared__ int sums2[4];
+  if ((threadIdx.x & 31) == 0) {
+    sums[threadIdx.x >> 5] = all;
+    sums2[threadIdx.x >> 5] = before;
+  }
+  __syncthreads();
+  all = sums[0] + sums[1] + sums[2] + sums[3];
+  before = sums2[0] + sums2[1] + sums2[2] + sums2[3];
+  const int tiles = (cached_len(a, b) + kTTile - 1) / kTTile + nodes;
+  const int64_t total = static_cast<int64_t>(all) * per;
+  const int64_t w = static_cast<int64_t>(before) * per + static_cast<int64_t>(unit) * tiles;
+  const int pieces = static_cast<int>(min(static_cast<int64_t>(ctas), total));
+  const int c0 = piece_of(total, w, pieces), c1 = piece_of(total, w + tiles - 1, pieces);
+  if (c0 == c1) return;
+  const int h = unit / a.groups, row0 = unit % a.groups * kTRows, rows = a.N * g;
+  for (int idx = threadIdx.x; idx < kTRows * D; idx += 128) {
+    const int r = idx / D, d = idx % D, rr = row0 + r;
+    if (rr >= rows) break;
+    auto part = [&](int c) { return a.ws + ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * kTRows + r) * (2 + D); };
+    float M = -INFINITY;
+    bool dead = false;
+    for (int c = c0; c <= c1; ++c) {
+      M = fmaxf(M, ld_act_f32(part(c)));
+      dead |= ld_act_f32(part(c) + 1) < 0.f;
+    }
+    float L = 0.f, O = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      const float f = rescale(ld_act_f32(part(c)), M);
+      L += ld_act_f32(part(c) + 1) * f;
+      O += ld_act_f32(part(c) + 2 + d) * f;
+    }
+    a.out[b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d] =
+        float_to_bf16_bits(dead ? 0.f : normalised(O, L));
+  }
+}
+
+}  // namespace iron
+
+using namespace iron;
+
+static int tree_pieces() { return sm_count() * kTCtasPerSm; }
+
+extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return static_cast<size_t>(tree_pieces()) * 2 * kTRows * (2 + head_dim) * sizeof(float);
+}
+
+extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
+                              const int32_t *parents, uint16_t *out, int num_nodes, int num_heads,
+                              const int64_t *q_strides, const int64_t *kv_strides, const int64_t *out_strides,
+                              float scale, void *workspace, size_t workspace_bytes, unsigned flags, void *stream) {
+  const int chk = pool_geometry_check(c);
+  if (chk != IRON_OK) return chk;
+  if (!c->lens || !q || !k_new || !v_new || !parents || !out || !q_strides || !kv_strides || !out_strides || !workspace)
+    return IRON_ERR_NULL;
+  if (c->layers != 1 || num_nodes <= 0 || num_heads <= 0 || num_heads % c->kv_heads) return IRON_ERR_SHAPE;
+  const int g = num_heads / c->kv_heads;
+  if (num_nodes > kTMaxNodes || g > 16 || c->slots > kTMaxBatch) return IRON_ERR_UNSUPPORTED;
+  if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new)) return IRON_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] % 8 || kv_strides[i] % 8 || out_strides[i] % 8) return IRON_ERR_ALIGN;
+  if (workspace_bytes < iron_tree_attn_workspace_bytes(c->slots, num_nodes, num_heads, c->kv_heads, c->head_dim))
+    return IRON_ERR_WORKSPACE;
+  TreeArgs a = {};
+  a.q = q;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.k = c->k;
+  a.v = c->v;
+  a.table = c->page_table;
+  a.lens = c->lens;
+  a.parents = parents;
+  a.out = out;
+  a.ws = static_cast<float *>(workspace);
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = q_strides[i];
+    a.ks[i] = kv_strides[i];
+    a.os[i] = out_strides[i];
+  }
+  a.B = c->slots;
+  a.N = num_nodes;
+  a.Hq = num_heads;
+  a.Hkv = c->kv_heads;
+  a.groups = (num_nodes * g + kTRows - 1) / kTRows;
+  a.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  a.M = c->max_pages;
+  a.P = c->num_pages;
+  a.scale_log2 = scale * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool pdl = (flags & IRON_FLAG_PDL) != 0, wide = c->head_dim == 128;
+  const int pieces = tree_pieces();
+  int st = launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps), 0, s, pdl, a);
+  if (st != IRON_OK) return st;
+  return launch(wide ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv * a.groups), dim3(128), 0, s,
+                true, a, pieces);
+}

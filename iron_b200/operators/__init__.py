@@ -22,6 +22,12 @@ _OPERATOR_MODULES = {
     "StridedCopy": "strided_copy",
     "Repeat": "repeat",
     "DecodeAttention": "decode_attention",
+    "PageAppend": "paged_cache",
+    "PageFork": "paged_cache",
+    "PageCompact": "paged_cache",
+    "PagedKVCache": "paged_cache",
+    "TreeAttention": "tree_attention",
+    "PageSelectAttention": "page_select_attention",
 }
 
 _SUBPACKAGES = ("flm",)
