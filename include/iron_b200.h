@@ -480,7 +480,11 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * its values. q, out bf16 [batch, num_nodes, Hq, D], k_new, v_new bf16 [batch, num_nodes,
  * kv_heads, D] with element strides {batch, node, head} (3 int64 each, multiples of 8; kv
  * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024.
- * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split. */
+ * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split.
+ * From 33 rows (nodes x Hq / kv_heads) per kv head on it runs on the tcgen05 tensor cores;
+ * iron_tree_attn_status returns IRON_ERR_TIMEOUT if a bounded wait ran out there since the
+ * last reset (reset != 0 clears it); it synchronises the device. */
+int iron_tree_attn_status(int reset);
 size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
 int iron_tree_attn(const iron_page_pool *pool, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
                    const int32_t *parents, uint16_t *out, int num_nodes, int num_heads, const int64_t *q_strides,

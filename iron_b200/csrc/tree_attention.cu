@@ -8,88 +8,14 @@
 // the GPU. Lengths are read on the device, so ragged batches and tables wider than the
 // sequences balance all the same. A piece that ends inside a unit leaves its (max, sum,
 // output) as a partial; a second kernel joins them in order.
-#include "paged.cuh"
+#include "tree.cuh"
 
 namespace iron {
 
 constexpr int kTRows = 16;     // rows per unit
 constexpr int kTTile = 64;     // tokens per tile: 16 per warp
 constexpr int kTWarps = 4;
-constexpr int kTMaxBatch = 1024;
-constexpr int kTMaxNodes = 128;
 constexpr int kTCtasPerSm = 4;
-
-struct TreeArgs {
-  const uint16_t *q, *k_new, *v_new, *k, *v;
-  const int *table, *lens, *parents;
-  uint16_t *out;
-  float *ws;  // [CTAs][2][kTRows][2 + D] partial (max, sum, output)
-  int64_t qs[3], ks[3], os[3];  // element strides {batch, node, head}
-  int B, N, Hq, Hkv, groups /* row groups per (sequence, kv head) */, page_shift, M, P;
-  float scale_log2;
-};
-
-// Tiles of a sequence: its cached tokens, then its nodes.
-__device__ __forceinline__ int cached_len(const TreeArgs &a, int b) {
-  return min(max(ld_act_i32(a.lens + b), 0), a.M << a.page_shift);
-}
-
-// Exclusive prefix sum of the sequences' tile counts into pref[0 .. B].
-template <int kThreads>
-__device__ __forceinline__ void tile_prefix(const TreeArgs &a, int *pref, int *warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int nodes = (a.N + kTTile - 1) / kTTile;
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    int v = b < a.B ? (cached_len(a, b) + kTTile - 1) / kTTile + nodes : 0;
-    const int mine = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) warp_sums[warp] = v;
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += warp_sums[w];
-      total += warp_sums[w];
-    }
-    if (b < a.B) pref[b] = base + before + v - mine;
-    base += total;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) pref[a.B] = base;
-  __syncthreads();
-}
-
-// Piece c of `total` tiles over `ctas` pieces starts here.
-__device__ __forceinline__ int64_t piece_start(int64_t total, int c, int ctas) { return total * c / ctas; }
-// The piece that holds tile w.
-__device__ __forceinline__ int piece_of(int64_t total, int64_t w, int ctas) {
-  return static_cast<int>(((w + 1) * ctas - 1) / total);
-}
-
-// Node i's path as bits (128), or none and `used` false. parents in shared memory.
-__device__ __forceinline__ bool tree_path(const int *parents, int i, uint32_t (&bits)[kTMaxNodes / 32]) {
-#pragma unroll
-  for (int w = 0; w < kTMaxNodes / 32; ++w) bits[w] = 0;
-  int j = i;
-  while (true) {
-#pragma unroll
-    for (int w = 0; w < kTMaxNodes / 32; ++w)
-      if (j >> 5 == w) bits[w] |= 1u << (j & 31);
-    const int p = parents[j];
-    if (p == -1) return true;
-    if (p < 0 || p >= j) break;
-    j = p;
-  }
-#pragma unroll
-  for (int w = 0; w < kTMaxNodes / 32; ++w) bits[w] = 0;
-  return false;
-}
 
 template <int D>
 __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(TreeArgs a) {
@@ -107,9 +33,9 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
   float (*red_o)[kTRows][D] = reinterpret_cast<float (*)[kTRows][D]>(smem);
   pdl_launch_dependents();
   pdl_wait();
-  tile_prefix<32 * kTWarps>(a, pref, warp_sums);
-  const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
-  const int64_t total = static_cast<int64_t>(pref[a.B]) * per;
+  tile_prefix<32 * kTWarps, kTTile>(a, pref, warp_sums);
+  const int g = a.Hq / a.Hkv;
+  const int64_t total = static_cast<int64_t>(pref[a.B]) * a.Hkv * a.groups;
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));  // none is empty
   if (static_cast<int>(blockIdx.x) >= pieces) return;
   int64_t w = piece_start(total, blockIdx.x, pieces);
@@ -117,18 +43,8 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
   const int page = 1 << a.page_shift;
 
   while (w < w_end) {
-    // the unit that holds tile w: the last sequence that starts at or before it
-    const int x = static_cast<int>(w / per);
-    int lo = 0, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pref[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    const int b = lo, tiles = pref[b + 1] - pref[b];
-    const int64_t rem = w - static_cast<int64_t>(pref[b]) * per;
-    const int unit = static_cast<int>(rem / tiles), first = static_cast<int>(rem % tiles);
-    const int count = static_cast<int>(min(static_cast<int64_t>(tiles - first), w_end - w));
-    const int h = unit / a.groups, row0 = unit % a.groups * kTRows;
+    const Segment sg = find_segment(a, pref, w, w_end);
+    const int b = sg.b, h = sg.h, row0 = sg.group * kTRows, first = sg.first, count = sg.count;
     const int len = cached_len(a, b), ctiles = (len + kTTile - 1) / kTTile;
     const int *table = a.table + static_cast<int64_t>(b) * a.M;
 
@@ -223,7 +139,7 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
       *reinterpret_cast<float2 *>(&red_o[warp][gid + 8][8 * j + 2 * tid]) = make_float2(at.o[j][2], at.o[j][3]);
     }
     __syncthreads();
-    const bool whole = count == tiles;
+    const bool whole = count == sg.tiles;
     const bool has_tree = first + count > ctiles;
     float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * kTRows * (2 + D);
     for (int idx = threadIdx.x; idx < kTRows * D; idx += 32 * kTWarps) {
@@ -262,37 +178,12 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
 // whole have nothing to join.
 template <int D>
 __global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a, int ctas) {
-  __shared__ int sums[4];
   pdl_launch_dependents();
   pdl_wait();
   const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
   const int b = blockIdx.x / per, unit = blockIdx.x % per;
-  const int nodes = (a.N + kTTile - 1) / kTTile;
-  // tiles before this sequence and in all
-  int before = 0, all = 0;
-  for (int i = threadIdx.x; i < a.B; i += 128) {
-    const int t = (cached_len(a, i) + kTTile - 1) / kTTile + nodes;
-    all += t;
-    if (i < b) before += t;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  __shared__ int sums2[4];
-  if ((threadIdx.x & 31) == 0) {
-    sums[threadIdx.x >> 5] = all;
-    sums2[threadIdx.x >> 5] = before;
-  }
-  __syncthreads();
-  all = sums[0] + sums[1] + sums[2] + sums[3];
-  before = sums2[0] + sums2[1] + sums2[2] + sums2[3];
-  const int tiles = (cached_len(a, b) + kTTile - 1) / kTTile + nodes;
-  const int64_t total = static_cast<int64_t>(all) * per;
-  const int64_t w = static_cast<int64_t>(before) * per + static_cast<int64_t>(unit) * tiles;
-  const int pieces = static_cast<int>(min(static_cast<int64_t>(ctas), total));
-  const int c0 = piece_of(total, w, pieces), c1 = piece_of(total, w + tiles - 1, pieces);
+  const UnitSpan sp = find_span<128, kTTile>(a, b, unit, ctas);
+  const int c0 = sp.c0, c1 = sp.c1;
   if (c0 == c1) return;
   const int h = unit / a.groups, row0 = unit % a.groups * kTRows, rows = a.N * g;
   for (int idx = threadIdx.x; idx < kTRows * D; idx += 128) {
@@ -324,7 +215,22 @@ static int tree_pieces() { return sm_count() * kTCtasPerSm; }
 
 extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
   if (batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  return static_cast<size_t>(tree_pieces()) * 2 * kTRows * (2 + head_dim) * sizeof(float);
+  const size_t few = static_cast<size_t>(tree_pieces()) * 2 * kTRows * (2 + head_dim) * sizeof(float);
+  const size_t many = tree_tc_workspace(head_dim);
+  return few > many ? few : many;
+}
+
+// Rows of a (sequence, kv head) from which the tensor cores' 128-row tiles are used.
+constexpr int kTensorRows = 33;
+
+// The tcgen05 form takes positive scales that do not vanish in log2 units, and new rows
+// whose strides TMA takes (not 0: broadcast views go to the other form).
+static bool use_tensor_form(const TreeArgs &a) {
+  for (int i = 0; i < 3; ++i) {
+    const int n = i == 0 ? a.B : i == 1 ? a.N : a.Hkv;
+    if (n > 1 && (a.ks[i] <= 0 || a.ks[i] >= (1LL << 38))) return false;
+  }
+  return a.N * (a.Hq / a.Hkv) >= kTensorRows && a.scale_log2 >= 1e-30f;
 }
 
 extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
@@ -370,6 +276,7 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.scale_log2 = scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool pdl = (flags & IRON_FLAG_PDL) != 0, wide = c->head_dim == 128;
+  if (use_tensor_form(a)) return tree_tc_launch(a, c->head_dim, pdl, s);
   const int pieces = tree_pieces();
   int st = launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps), 0, s, pdl, a);
   if (st != IRON_OK) return st;

@@ -1,0 +1,651 @@
+// Tree attention on the 5th-generation tensor cores, for many rows per kv head.
+//
+// Rows: num_nodes * group rows of a (sequence, kv head) read the same K and V; a unit is up
+// to 256 of them, a tile is 128 tokens. One CTA per SM takes an equal share of all units'
+// tiles (tree.cuh). Two streams of 128 rows run staggered, so that one's softmax overlaps
+// the other's MMAs: with more than 128 rows stream s is the unit's rows 128 s ... and both
+// see every tile; with fewer, both hold the same rows and stream s sees every second tile;
+// stream 0 then joins both results, whose rows lie in the same TMEM lanes.
+//
+// Warps: 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns one row: no shuffles), 8
+// issues the MMAs, 9 loads (TMA, one box per page and 64 columns).
+//   S = Q K^T     128 x 128 x D, both operands in shared memory (K-major)
+//   P -> TMEM     over S: bf16 hi and lo parts, 64 columns each (P = hi + lo to 2^-16: one
+//                 bf16 would double the error of the rounded output)
+//   O += P V      128 x D x 128, twice; A from TMEM, V as it lies in the page (MN-major)
+// TMEM: S0, S1 128 columns each, O0, O1 D each. O is rescaled only when a row's maximum
+// has grown by more than 2^8 (P stays below 2^8, exact in the sums' fp32 range).
+//
+// Bounds: D = 128: per tile and stream 512 cycles of S and 1024 of P V against 1024 of ex2
+// (16 per cycle and SM), so the tensor cores; D = 64: ex2. What a tile must not hold (past
+// the length, unused nodes) is masked in S and zeroed in V.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "tc.cuh"
+#include "tree.cuh"
+
+namespace iron {
+namespace gemm {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // gemm_tc.cu
+}
+
+__device__ unsigned g_tree_status;  // 0 = ok, else the first failing role's code
+
+namespace treetc {
+
+constexpr int kTile = 128;
+constexpr int kThreads = 384;  // three warpgroups; warps 10 and 11 idle
+// registers: 384 x 168 at launch = 2 x 128 x 216 (a row of S is 128 of them) + 128 x 72
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
+static_assert(kThreads * 168 == 256 * kSoftmaxRegs + 128 * kOtherRegs, "the split must not exceed the launch's registers");
+constexpr int kMasks = 8;  // tiles' masks in flight: stages + 2 at least
+constexpr uint64_t kDeadline = 2000000000ull;  // per wait, ns
+
+template <int D>
+struct Cfg {
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kPanels = D / 64;
+  static constexpr uint32_t kPanel = kTile * 128;          // 128 rows x 64 bf16
+  static constexpr uint32_t kOperand = kPanels * kPanel;   // Q tile, K tile or V tile
+  static constexpr uint32_t kSmem = 1024 + 2 * kOperand + 2 * kStages * kOperand;
+  static constexpr int kPart = kTile * D + 2 * kTile;      // floats of one stream's partial: O, then (m, l)
+};
+
+struct Bars {  // mbarrier addresses
+  uint32_t base;
+  template <int S> __device__ uint32_t kfull(int i) const { return base + 8 * i; }
+  template <int S> __device__ uint32_t kempty(int i) const { return base + 8 * (S + i); }
+  template <int S> __device__ uint32_t vfull(int i) const { return base + 8 * (2 * S + i); }
+  template <int S> __device__ uint32_t vempty(int i) const { return base + 8 * (3 * S + i); }
+  template <int S> __device__ uint32_t sfull(int i) const { return base + 8 * (4 * S + i); }
+  template <int S> __device__ uint32_t pfull(int i) const { return base + 8 * (4 * S + 2 + i); }
+  template <int S> __device__ uint32_t ofull(int i) const { return base + 8 * (4 * S + 4 + i); }
+  template <int S> __device__ uint32_t qfull(int i) const { return base + 8 * (4 * S + 6 + i); }
+  template <int S> __device__ uint32_t odd() const { return base + 8 * (4 * S + 8); }
+  template <int S> __device__ uint32_t drain() const { return base + 8 * (4 * S + 9); }
+  template <int S> __device__ uint32_t other() const { return base + 8 * (4 * S + 10); }
+  template <int S> __device__ uint32_t joined() const { return base + 8 * (4 * S + 11); }
+};
+
+struct Maps {
+  CUtensorMap k, v, k_new, v_new;
+};
+
+// Tiles of a segment that stream s handles, and the segment's form.
+struct Streams {
+  bool both;  // both streams see every tile (more than 128 rows)
+  int n[2];
+};
+__device__ __forceinline__ Streams streams_of(const TreeArgs &a, const Segment &sg) {
+  const int rows = a.N * (a.Hq / a.Hkv) - sg.group * 256;
+  Streams st;
+  st.both = rows > 128;
+  st.n[0] = st.both ? sg.count : (sg.count + 1) / 2;
+  st.n[1] = st.both ? sg.count : sg.count / 2;
+  return st;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
+  using C = Cfg<D>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_store[4 * S + 12];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int pref[kTMaxBatch + 1], warp_sums[kThreads / 32];
+  __shared__ uint32_t masks[kMasks][4];
+  __shared__ int parents_s[8][kTMaxNodes];  // per softmax warp
+  __shared__ float2 other_ml[kTile];        // (m, l) of stream 1, for the join of both streams
+  __shared__ int odd_flag;                  // V of the tree held values that are not finite
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (base - raw);
+  const uint32_t q0 = base, k0 = base + 2 * C::kOperand, v0 = k0 + S * C::kOperand;
+  const Bars bars{smem_addr(bar_store)};
+
+  pdl_launch_dependents();
+  pdl_wait();
+  tile_prefix<kThreads, kTile>(a, pref, warp_sums);
+  const int64_t total = static_cast<int64_t>(pref[a.B]) * a.Hkv * a.groups;
+  const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));  // none is empty
+  if (static_cast<int>(blockIdx.x) >= pieces) return;
+  const int64_t w_begin = piece_start(total, blockIdx.x, pieces), w_end = piece_start(total, blockIdx.x + 1, pieces);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4 * S; ++i) tc::mbar_init_u32(bars.base + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init_u32(bars.sfull<S>(i), 1);
+      tc::mbar_init_u32(bars.pfull<S>(i), 4);
+      tc::mbar_init_u32(bars.ofull<S>(i), 1);
+      tc::mbar_init_u32(bars.qfull<S>(i), 4);
+    }
+    tc::mbar_init_u32(bars.odd<S>(), 4);
+    tc::mbar_init_u32(bars.drain<S>(), 1);
+    tc::mbar_init_u32(bars.other<S>(), 4);
+    tc::mbar_init_u32(bars.joined<S>(), 4);
+    odd_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 8) tc::tmem_alloc(smem_addr(&tmem_slot), 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int g = a.Hq / a.Hkv, rows_all = a.N * g;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 9) {
+    // ---- loads ----
+    if (lane == 0) {
+      tc::prefetch_tmap(&maps.k);
+      tc::prefetch_tmap(&maps.v);
+    }
+    const int page = 1 << a.page_shift, ppt = kTile >> a.page_shift;  // pages per tile
+    bool ok = true;
+    int it = 0;
+    for (int64_t w = w_begin; w < w_end && ok;) {
+      const Segment sg = find_segment(a, pref, w, w_end);
+      const int len = cached_len(a, sg.b), ctiles = (len + kTile - 1) / kTile;
+      const int *table = a.table + static_cast<int64_t>(sg.b) * a.M;
+      // 32 table entries at a time, the next ones requested while these are used
+      const int per = 32 >> (7 - a.page_shift);  // tiles per 32 entries
+      auto entries = [&](int tile) {
+        const int e = tile * ppt + lane;
+        return e < a.M ? ld_act_i32(table + e) : -1;
+      };
+      int cur = entries(sg.first), next = entries(sg.first + per), used = 0;
+      for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
+        const int s = it % S;
+        const bool tree = i >= ctiles;
+        // this tile's pages: lane l < ppt holds page l and its valid rows
+        if (used == per) {
+          cur = next;
+          next = entries(i + per);
+          used = 0;
+        }
+        const int pid = __shfl_sync(0xffffffffu, cur, (used * ppt + lane) & 31);
+        ++used;
+        int n = 0;
+        if (!tree && lane < ppt && pid >= 0 && pid < a.P) n = max(0, min(page, len - i * kTile - lane * page));
+        uint32_t bits = 0;  // lane w < 4: the valid tokens of word w
+        for (int p = 0; p < ppt; ++p) {
+          const int np = __shfl_sync(0xffffffffu, n, p);
+          const int lo = max(p * page, 32 * lane), hi = min(p * page + np, 32 * lane + 32);
+          if (hi > lo) bits |= (hi - lo == 32 ? 0xffffffffu : (1u << (hi - lo)) - 1u) << (lo & 31);
+        }
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, n > 0));
+        const uint32_t bytes = tree ? C::kOperand : boxes * page * D * 2;
+        const uint32_t parity = ((it / S) & 1) ^ 1;
+        ok = __all_sync(0xffffffffu, tc::wait_until(bars.kempty<S>(s), parity, kDeadline));
+        if (!ok) break;
+        if (lane < 4) masks[it % kMasks][lane] = bits;
+        __syncwarp();
+        if (lane == 0) tc::expect_tx(bars.kfull<S>(s), bytes);
+        __syncwarp();
+        auto load = [&](const CUtensorMap *pages, const CUtensorMap *fresh, uint32_t dst, uint32_t bar) {
+          if (tree) {
+            if (lane < C::kPanels) tc::tma_load_4d(dst + lane * C::kPanel, fresh, lane * 64, 0, sg.h, sg.b, bar);
+          } else if (n > 0) {
+#pragma unroll
+            for (int c = 0; c < C::kPanels; ++c)
+              tc::tma_load_4d(dst + c * C::kPanel + lane * page * 128, pages, c * 64, 0, sg.h, pid, bar);
+          }
+        };
+        load(&maps.k, &maps.k_new, k0 + s * C::kOperand, bars.kfull<S>(s));
+        ok = __all_sync(0xffffffffu, tc::wait_until(bars.vempty<S>(s), parity, kDeadline));
+        if (!ok) {
+          // this tile's K is on its way already: let it land
+          tc::wait_until(bars.kfull<S>(s), (it / S) & 1, 100000000ull);
+          break;
+        }
+        if (lane == 0) tc::expect_tx(bars.vfull<S>(s), bytes);
+        __syncwarp();
+        load(&maps.v, &maps.v_new, v0 + s * C::kOperand, bars.vfull<S>(s));
+      }
+      w += sg.count;
+    }
+    if (!ok) {
+      if (lane == 0) atomicCAS(&g_tree_status, 0u, 1u);
+      // copies in flight land before the CTA's shared memory goes away
+      for (int j = max(0, it - S); j < it; ++j) {
+        tc::wait_until(bars.kfull<S>(j % S), (j / S) & 1, 100000000ull);
+        tc::wait_until(bars.vfull<S>(j % S), (j / S) & 1, 100000000ull);
+      }
+    }
+    } else if (warp == 8) {
+    // ---- MMAs, one thread ----
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, kTile);
+      constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
+      bool ok = true;
+      int it0 = 0;
+      uint32_t pc[2] = {0, 0}, qc[2] = {0, 0};
+      for (int64_t w = w_begin; w < w_end && ok;) {
+        const Segment sg = find_segment(a, pref, w, w_end);
+        const Streams st = streams_of(a, sg);
+        auto tile_of = [&](int s, int j) { return it0 + (st.both ? j : 2 * j + s); };
+        auto scores = [&](int s, int j) {
+          const int it = tile_of(s, j), slot = it % S;
+          ok = ok && tc::wait_until(bars.kfull<S>(slot), (it / S) & 1, kDeadline);
+          if (!ok) return;
+          tc::fence_after_sync();
+          // a step of the start address is a step of the descriptor's low bits (16-byte units)
+          const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
+          const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand);
+#pragma unroll 1
+          for (int c = 0; c < C::kPanels; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::mma_bf16(tmem + s * 128, q + c * (C::kPanel >> 4) + kk * 2, k + c * (C::kPanel >> 4) + kk * 2, idesc_s,
+                           c > 0 || kk > 0);
+          tc::mma_commit(bars.sfull<S>(s));
+          if (!st.both || s == 1) tc::mma_commit(bars.kempty<S>(slot));
+        };
+        auto values = [&](int s, int j) {
+          const int it = tile_of(s, j), slot = it % S;
+          ok = ok && tc::wait_until(bars.pfull<S>(s), pc[s]++ & 1, kDeadline) &&
+               tc::wait_until(bars.vfull<S>(slot), (it / S) & 1, kDeadline);
+          if (!ok) return;
+          tc::fence_after_sync();
+          const uint32_t p = tmem + s * 128, o = tmem + 256 + s * D;
+          const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand, C::kPanel);
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              tc::mma_bf16_ts(o, p + part * 64 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || part > 0 || kk > 0);
+          if (!st.both || s == 1) tc::mma_commit(bars.vempty<S>(slot));
+          if (j == st.n[s] - 1) tc::mma_commit(bars.ofull<S>(s));
+        };
+        for (int s = 0; s < 2; ++s)
+          if (st.n[s] > 0 && ok) {
+            ok = tc::wait_until(bars.qfull<S>(s), qc[s]++ & 1, kDeadline);
+            if (ok) scores(s, 0);
+          }
+        for (int j = 0; j < st.n[0] && ok; ++j)
+          for (int s = 0; s < 2; ++s)
+            if (j < st.n[s]) {
+              if (ok) values(s, j);
+              if (ok && j + 1 < st.n[s]) scores(s, j + 1);
+            }
+        it0 += sg.count;
+        w += sg.count;
+      }
+      if (!ok) atomicCAS(&g_tree_status, 0u, 2u);
+      // every MMA issued is done before TMEM is freed
+      tc::mma_commit(bars.drain<S>());
+      tc::wait_until(bars.drain<S>(), 0, kDeadline);
+    }
+    __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ---- softmax of one stream: thread = row ----
+    const int s = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
+    uint8_t *qs = smem + s * C::kOperand;
+    int *parents = parents_s[warp];
+    bool ok = true;
+    int it0 = 0;
+    uint32_t sc = 0, oc = 0, fc = 0, jc = 0;
+    for (int64_t w = w_begin; w < w_end && ok;) {
+      const Segment sg = find_segment(a, pref, w, w_end);
+      const Streams st = streams_of(a, sg);
+      const int b = sg.b, h = sg.h, n = st.n[s];
+      const int len = cached_len(a, b), ctiles = (len + kTile - 1) / kTile;
+      const bool has_tree = sg.first + sg.count > ctiles;
+      const int row = sg.group * 256 + (st.both ? s * 128 : 0) + r;
+      const bool live = row < rows_all;
+      const int node = live ? row / g : 0, hq = h * g + (live ? row % g : 0);
+      float m = -INFINITY, l = 0.f;
+      uint32_t path[4] = {0, 0, 0, 0};
+      if (n > 0) {
+        // the row of Q, swizzled as TMA would write it: 16-byte piece c of row r at c ^ (r % 8)
+        const uint16_t *q = a.q + b * a.qs[0] + node * a.qs[1] + hq * a.qs[2];
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = live ? ld_act_v4(q + c * 8) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(qs + (c >> 3) * C::kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
+        if (has_tree) {
+          for (int i = lane; i < kTMaxNodes; i += 32)
+            parents[i] = i < a.N ? ld_act_i32(a.parents + static_cast<int64_t>(b) * a.N + i) : -2;
+          __syncwarp();
+          if (live) tree_path(parents, node, path);
+        }
+        tc::fence_proxy_async_smem();
+        tc::fence_before_sync();  // the last segment's O has been read
+        __syncwarp();
+        if (lane == 0) tc::arrive(bars.qfull<S>(s));
+      }
+      for (int j = 0; j < n; ++j) {
+        const int i = sg.first + (st.both ? j : 2 * j + s), it = it0 + i - sg.first, slot = it % S;
+        ok = __all_sync(0xffffffffu, tc::wait_until(bars.sfull<S>(s), sc++ & 1, kDeadline) &&
+                                         tc::wait_until(bars.kfull<S>(slot), (it / S) & 1, kDeadline));
+        if (!ok) break;
+        tc::fence_after_sync();
+        uint32_t x[128];
+        tc::tmem_ld64(ts, x);
+        tc::tmem_ld64(ts + 64, x + 64);
+        const bool tree = i >= ctiles;
+        uint32_t see[4];
+        bool all = true;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t valid = masks[it % kMasks][q];
+          see[q] = tree ? path[q] : valid;
+          all = all && valid == 0xffffffffu;
+        }
+        if (tree || !all) {  // the same for all threads
+#pragma unroll
+          for (int t = 0; t < 128; ++t)
+            if (!(see[t >> 5] >> (t & 31) & 1u)) x[t] = 0xff800000u;  // -inf
+          if (!st.both || s == 0) {
+            // row r of V: zero where the tile holds nothing, and where a node's value is not
+            // finite (0 * inf is not 0; rows that see it get it added at the end)
+            ok = __all_sync(0xffffffffu, tc::wait_until(bars.vfull<S>(slot), (it / S) & 1, kDeadline));
+            if (!ok) break;
+            bool keep;
+            if (tree) {
+              uint32_t unused[4];
+              keep = r < a.N && tree_path(parents, r, unused);
+            } else {
+              keep = masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
+            }
+            uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              uint4 *e = reinterpret_cast<uint4 *>(vrow + (c >> 3) * C::kPanel + ((c & 7) << 4));
+              if (!keep) {
+                *e = make_uint4(0, 0, 0, 0);
+              } else if (tree) {
+                uint4 y = *e;
+                uint32_t *u = reinterpret_cast<uint32_t *>(&y);
+                bool change = false;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u, change = true;
+                  if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu, change = true;
+                }
+                if (change) {
+                  *e = y;
+                  odd = true;
+                }
+              }
+            }
+            if (odd) atomicExch(&odd_flag, 1);
+            tc::fence_proxy_async_smem();
+            if (tree && st.both) {
+              __syncwarp();
+              if (lane == 0) tc::arrive(bars.odd<S>());
+            }
+          }
+        }
+        // the row's maximum, its factor and the probabilities
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < 128; ++t) mx[t & 3] = fmaxf(mx[t & 3], __uint_as_float(x[t]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool grow = top > m + 8.f || (m == -INFINITY && top != -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float to_m = grow ? top : m;
+            const float f = grow ? ex2_approx(m - to_m) : 1.f;  // ex2(-inf) = 0: nothing seen before
+            l *= f;
+            m = to_m;
+            // P V of the tile before is complete: S was issued after it
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              asm volatile(
+                  "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                  "tcgen05.wait::ld.sync.aligned;"
+                  : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                    "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                  : "r"(to + c)
+                  : "memory");
+#pragma unroll
+              for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+              tc::tmem_st16(to + c, o);
+            }
+          }
+        }
+        float ref = m == -INFINITY ? 0.f : m, by = a.scale_log2;
+        // past 2^20 the fused product below would keep digits that m has lost: round it first
+        if (__any_sync(0xffffffffu, fabsf(ref) > 1048576.f)) {
+#pragma unroll
+          for (int t = 0; t < 128; ++t) x[t] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[t]), by), ref));
+          ref = 0.f;
+          by = 1.f;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(x[32 * c + 2 * q]), by, -ref));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(x[32 * c + 2 * q + 1]), by, -ref));
+            sum[q & 1] += p0;
+            sum[2 + (q & 1)] += p1;
+            hi[q] = pack_bf16x2(p0, p1);
+            lo[q] = pack_bf16x2(p0 - bf16_lo(hi[q]), p1 - bf16_hi(hi[q]));
+          }
+          tc::tmem_st16(ts + 16 * c, hi);
+          tc::tmem_st16(ts + 64 + 16 * c, lo);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_st_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::arrive(bars.pfull<S>(s));
+      }
+      if (!ok) break;
+      // ---- the segment's result ----
+      const bool direct = sg.count == sg.tiles, join = !st.both && st.n[1] > 0;
+      if (n > 0) ok = __all_sync(0xffffffffu, tc::wait_until(bars.ofull<S>(s), oc++ & 1, kDeadline));
+      if (!ok) break;
+      if (join && s == 1) {
+        other_ml[r] = make_float2(m, l);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::arrive(bars.other<S>());
+        // stream 0 reads this stream's O from TMEM before the next segment overwrites it
+        ok = __all_sync(0xffffffffu, tc::wait_until(bars.joined<S>(), jc++ & 1, kDeadline));
+        if (!ok) break;
+        tc::fence_after_sync();
+      } else if (n > 0) {
+        float f0 = 1.f, f1 = 0.f;
+        if (join) {
+          ok = __all_sync(0xffffffffu, tc::wait_until(bars.other<S>(), jc++ & 1, kDeadline));
+          if (!ok) break;
+          const float2 o = other_ml[r];
+          const float M = fmaxf(m, o.x);
+          f0 = rescale(m, M);
+          f1 = rescale(o.x, M);
+          l = l * f0 + o.y * f1;
+          m = M;
+        }
+        if (has_tree && st.both) {
+          ok = __all_sync(0xffffffffu, tc::wait_until(bars.odd<S>(), fc++ & 1, kDeadline));
+          if (!ok) break;
+        }
+        tc::fence_after_sync();
+        const bool dead = has_tree && (path[0] | path[1] | path[2] | path[3]) == 0;
+        const bool odd = has_tree && *reinterpret_cast<volatile int *>(&odd_flag) != 0;
+        const float inv = l == 0.f || dead ? 0.f : 1.f / l;
+        uint16_t *dst = a.out + b * a.os[0] + node * a.os[1] + hq * a.os[2];
+        float *part = a.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + (sg.first == 0 ? 1 : 0)) * 2 + s) * C::kPart;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tc::tmem_ld32(to + c, o);
+          if (join) {
+            uint32_t o1[32];
+            tc::tmem_ld32(to + D + c, o1);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + __uint_as_float(o1[e]) * f1);
+          }
+          if (odd && live)
+            for (int j = 0; j < a.N; ++j) {
+              if (!(path[j >> 5] >> (j & 31) & 1u)) continue;
+              const uint16_t *v = a.v_new + b * a.ks[0] + j * a.ks[1] + h * a.ks[2] + c;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float f = bf16_bits_to_float(ld_act_u16(v + e));
+                if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+              }
+            }
+          if (direct) {
+            if (live)
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint32_t y[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  // a row that saw nothing (l = 0) or an unused node is zero
+                  const float f0 = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * q]) * inv;
+                  const float f1 = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * q + 1]) * inv;
+                  y[q] = pack_bf16x2(f0, f1);
+                }
+                *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4 *>(part + r * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (!direct) {
+          part[kTile * D + 2 * r] = m;
+          part[kTile * D + 2 * r + 1] = dead ? -1.f : l;  // -1: the join kernel writes zeros
+        }
+        if (join) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::arrive(bars.joined<S>());
+        }
+      }
+      it0 += sg.count;
+      w += sg.count;
+    }
+    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 3u + s);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 8) tc::tmem_free(tmem, 512);
+}
+
+// Joins the partials of 16 rows of one unit: 256 threads, D / 4 float4 columns x rows.
+template <int D>
+__global__ void __launch_bounds__(256) tree_tc_join_kernel(TreeArgs a, int ctas) {
+  using C = Cfg<D>;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
+  const int b = blockIdx.x / per, unit = blockIdx.x % per, h = unit / a.groups, group = unit % a.groups;
+  const int rows = min(256, a.N * g - group * 256);
+  if (static_cast<int>(blockIdx.y) * 16 >= rows) return;
+  const UnitSpan sp = find_span<256, kTile>(a, b, unit, ctas);
+  if (sp.c0 == sp.c1) return;  // written by the piece that held it
+  for (int idx = threadIdx.x; idx < 16 * D / 4; idx += 256) {
+    const int ru = blockIdx.y * 16 + idx / (D / 4), d = idx % (D / 4) * 4;
+    if (ru >= rows) break;
+    const int r = ru % 128, s = ru / 128;
+    auto part = [&](int c) { return a.ws + ((static_cast<int64_t>(c) * 2 + (c == sp.c0 ? 1 : 0)) * 2 + s) * C::kPart; };
+    float M = -INFINITY;
+    bool dead = false;
+    for (int c = sp.c0; c <= sp.c1; ++c) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(c) + kTile * D + 2 * r));
+      M = fmaxf(M, ml.x);
+      dead |= ml.y < 0.f;
+    }
+    float L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = sp.c0; c <= sp.c1; ++c) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(c) + kTile * D + 2 * r));
+      const float4 o = __ldcg(reinterpret_cast<const float4 *>(part(c) + r * D + d));
+      const float f = rescale(ml.x, M);
+      L += ml.y * f;
+      O[0] += o.x * f;
+      O[1] += o.y * f;
+      O[2] += o.z * f;
+      O[3] += o.w * f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
+    const int row = group * 256 + ru;
+    *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d) =
+        make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
+  }
+}
+
+static int make_map(CUtensorMap *m, const void *ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], int rows) {
+  auto fn = gemm::encode_fn();
+  if (!fn) return IRON_ERR_UNSUPPORTED;
+  cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(ptr), d, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? IRON_OK
+             : IRON_ERR_ARG;
+}
+
+template <int D>
+static int launch_tc(TreeArgs a, bool pdl, cudaStream_t s) {
+  using C = Cfg<D>;
+  static PerDeviceOnce once;
+  const int st0 = once.run([] {
+    return call_status(cudaFuncSetAttribute(tree_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  });
+  if (st0 != IRON_OK) return st0;
+  a.groups = (a.N * (a.Hq / a.Hkv) + 255) / 256;
+  Maps maps;
+  const uint64_t page = 1ull << a.page_shift, B = a.B, N = a.N, H = a.Hkv;
+  const uint64_t pd[4] = {D, page, H, static_cast<uint64_t>(a.P)}, ps[3] = {D * 2, page * D * 2, H * page * D * 2};
+  // a dimension of one element may have any stride: give TMA one that it takes
+  auto step = [](int64_t stride, uint64_t n) { return n > 1 ? static_cast<uint64_t>(stride) * 2 : 16ull; };
+  const uint64_t nd[4] = {D, N, H, B}, ns[3] = {step(a.ks[1], N), step(a.ks[2], H), step(a.ks[0], B)};
+  int st = make_map(&maps.k, a.k, pd, ps, static_cast<int>(page));
+  if (st == IRON_OK) st = make_map(&maps.v, a.v, pd, ps, static_cast<int>(page));
+  if (st == IRON_OK) st = make_map(&maps.k_new, a.k_new, nd, ns, kTile);
+  if (st == IRON_OK) st = make_map(&maps.v_new, a.v_new, nd, ns, kTile);
+  if (st != IRON_OK) return st;
+  const int ctas = sm_count();
+  st = launch(tree_tc_kernel<D>, dim3(ctas), dim3(kThreads), C::kSmem, s, pdl, maps, a);
+  if (st != IRON_OK) return st;
+  const int rows = a.N * (a.Hq / a.Hkv);
+  return launch(tree_tc_join_kernel<D>, dim3(a.B * a.Hkv * a.groups, ((rows < 256 ? rows : 256) + 15) / 16), dim3(256), 0, s,
+                true, a, ctas);
+}
+
+}  // namespace treetc
+
+size_t tree_tc_workspace(int head_dim) {
+  const size_t part = head_dim == 128 ? treetc::Cfg<128>::kPart : treetc::Cfg<64>::kPart;
+  return static_cast<size_t>(sm_count()) * 4 * part * sizeof(float);
+}
+
+int tree_tc_launch(TreeArgs a, int head_dim, bool pdl, cudaStream_t s) {
+  return head_dim == 128 ? treetc::launch_tc<128>(a, pdl, s) : treetc::launch_tc<64>(a, pdl, s);
+}
+
+}  // namespace iron
+
+extern "C" int iron_tree_attn_status(int reset) {
+  unsigned v = 0;
+  if (cudaMemcpyFromSymbol(&v, iron::g_tree_status, sizeof(v)) != cudaSuccess) return iron::launch_status();
+  if (reset) {
+    const unsigned z = 0;
+    if (cudaMemcpyToSymbol(iron::g_tree_status, &z, sizeof(z)) != cudaSuccess) return iron::launch_status();
+  }
+  return v ? IRON_ERR_TIMEOUT : IRON_OK;
+}
