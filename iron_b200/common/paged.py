@@ -68,36 +68,50 @@ class PagedOperator(MLIROperator):
         if len(bufs) != len(self._wanted):
             raise ValueError(f"{type(self).__name__} takes {len(self._wanted)} buffers, got {len(bufs)}")
         for i, (t, (numel, dtype, shape, strided)) in enumerate(zip(bufs, self._wanted)):
-            t = getattr(t, "device_tensor", t)
+            if not isinstance(t, torch.Tensor):
+                t = t.device_tensor
             if t.dtype is not dtype:
                 raise ValueError(f"buffer {i} of {type(self).__name__} is {t.dtype}, needs {dtype}")
-            if strided and t.shape == shape:
-                if t.stride(-1) != 1:
-                    raise ValueError(f"buffer {i} of {type(self).__name__} needs a contiguous last dimension")
-                continue
-            if t.numel() < numel:
-                raise ValueError(f"buffer {i} of {type(self).__name__} holds {t.numel()} values, needs {numel}")
-            if not t.is_contiguous():
+            if t.is_contiguous():
+                if t.numel() < numel:
+                    raise ValueError(f"buffer {i} of {type(self).__name__} holds {t.numel()} values, needs {numel}")
+            elif not strided or t.shape != shape:
                 raise ValueError(f"buffer {i} of {type(self).__name__} must be contiguous")
+            elif t.stride(-1) != 1:
+                raise ValueError(f"buffer {i} of {type(self).__name__} needs a contiguous last dimension")
 
     def get_callable(self):
+        import torch
+
         _lib.load()
         written = [i for i, s in enumerate(self.get_arg_spec()) if s.direction != "in"]
+        check, launch, device = self._check_buffers, self._launch, torch.cuda.current_device
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
         def call(*bufs):
-            self._check_buffers(bufs)
-            self._launch(*bufs, stream=_lib.current_stream())
+            check(bufs)
+            launch(*bufs, stream=raw(device()))
             for i in written:
-                if hasattr(bufs[i], "mark_device_written"):
+                if not isinstance(bufs[i], torch.Tensor):
                     bufs[i].mark_device_written()
 
         return call
 
 
+def address(t):
+    """Device address of a CUDA tensor (or of an iron_b200 Tensor)."""
+    try:
+        if t.is_cuda:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    return _lib.dptr(t)
+
+
 def strides(t, shape):
     """Element strides of the leading dimensions of `t` seen as `shape`."""
     t = getattr(t, "device_tensor", t)
-    if tuple(t.shape) == tuple(shape):
+    if t.shape == shape:
         return t.stride()[:-1]
     out, step = [], 1
     for n in reversed(shape[1:]):

@@ -223,77 +223,69 @@ __global__ void __launch_bounds__(kPlanThreads) append_plan_kernel(AppendArgs a)
 
 // One CTA: one touched page of one slot, one layer, K or V. Threads are rows x 16-byte
 // columns of a token's Hkv * D values, so a thread's column (8 dims of one head) is fixed
-// and the bounds of a page that becomes full are folded into the same pass.
+// and the bounds of a page that becomes full are folded into the same pass (minimum and
+// maximum of bf16 pairs are exact in bf16).
+// The page's row numbers go through shared memory first, so that all of a thread's row
+// loads are independent; 3 CTAs per SM x 256 threads x 8 loads of 16 bytes are in flight.
+// B200, 16 layers, 4 prompts of up to 2048 tokens (402 MB moved): 107 us with the numbers
+// loaded per row and 2 CTAs per SM.
 constexpr int kAppendThreads = 256;
 
-__global__ void __launch_bounds__(kAppendThreads) append_write_kernel(AppendArgs a) {
-  extern __shared__ float bounds[];  // [row groups][2][Hkv * D] (pages that become full)
+template <bool kSummaries>
+__global__ void __launch_bounds__(kAppendThreads, 3) append_write_kernel(AppendArgs a) {
+  extern __shared__ __align__(16) uint16_t bounds[];  // [row groups][2][Hkv * D] (pages that become full)
+  __shared__ int rows_s[128];
   const int s = blockIdx.y, layer = blockIdx.z >> 1;
   const bool is_v = blockIdx.z & 1;
   pdl_launch_dependents();
   pdl_wait();
-  const int n = ld_act_i32(a.take + s);
-  if (n <= 0) return;
-  const int len = ld_act_i32(a.lens_out + s) - n;
+  const int n = ld_act_i32(a.take + s), end = ld_act_i32(a.lens_out + s), len = end - n;
   const int pi = len / a.page + blockIdx.x;           // the page's place in the slot
-  const int t0 = max(len, pi * a.page), t1 = min(len + n, (pi + 1) * a.page);
-  if (t0 >= t1) return;
+  const int t0 = max(len, pi * a.page), t1 = min(end, (pi + 1) * a.page);
+  if (n <= 0 || t0 >= t1) return;
   const int p = ld_act_i32(a.table + static_cast<int64_t>(s) * a.M + pi);
+  if (static_cast<int>(threadIdx.x) < t1 - t0)
+    rows_s[threadIdx.x] = ld_act_i32(a.index + static_cast<int64_t>(s) * a.N + t0 - len + threadIdx.x);
+  __syncthreads();
   const int vpr = a.Hkv * a.D / 8;                    // 16-byte columns per token
-  const int groups = min(kAppendThreads / min(vpr, kAppendThreads), 64);
-  const int width = min(vpr, kAppendThreads);
+  const int width = min(vpr, kAppendThreads), groups = min(kAppendThreads / width, 64);
   const int g = threadIdx.x / width, c0 = threadIdx.x % width;
-  const uint16_t *src = (is_v ? a.v_new : a.k_new) +
-                        (static_cast<int64_t>(layer) * a.S + s) * a.N * a.Hkv * a.D;
-  uint16_t *dst = (is_v ? a.v : a.k) + layer * a.layer_stride + static_cast<int64_t>(p) * a.Hkv * a.page * a.D;
-  const int *index = a.index + static_cast<int64_t>(s) * a.N;
-  const bool full = a.codes && !is_v && t1 == (pi + 1) * a.page;
   const int row = a.Hkv * a.D;
+  const uint16_t *src = (is_v ? a.v_new : a.k_new) + (static_cast<int64_t>(layer) * a.S + s) * a.N * row;
+  uint16_t *dst = (is_v ? a.v : a.k) + layer * a.layer_stride + static_cast<int64_t>(p) * row * a.page;
+  const bool full = kSummaries && !is_v && t1 == (pi + 1) * a.page;
+  const __nv_bfloat162 inf = __float2bfloat162_rn(INFINITY);
   for (int c = c0; c < vpr && g < groups; c += width) {
     const int h = c * 8 / a.D, d = c * 8 % a.D;
-    uint16_t *to = dst + static_cast<int64_t>(h) * a.page * a.D + d;
-    float lo[8], hi[8];
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+    uint16_t *to = dst + (static_cast<int64_t>(h) * a.page - pi * a.page) * a.D + d;
+    __nv_bfloat162 lo[4] = {inf, inf, inf, inf}, hi[4] = {__hneg2(inf), __hneg2(inf), __hneg2(inf), __hneg2(inf)};
     auto fold = [&](const uint4 &x) {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      const __nv_bfloat162 *w = reinterpret_cast<const __nv_bfloat162 *>(&x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
-        nan |= f != f;
-        lo[i] = fminf(lo[i], f);
-        hi[i] = fmaxf(hi[i], f);
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = __hmin2_nan(lo[i], w[i]);
+        hi[i] = __hmax2_nan(hi[i], w[i]);
       }
     };
     constexpr int kU = 8;
     for (int t = t0 + g; t < t1; t += kU * groups) {
       uint4 x[kU];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int tt = t + u * groups;
-        if (tt < t1) {
-          const int j = ld_act_i32(index + tt - len);
-          x[u] = ld_act_v4(src + static_cast<int64_t>(j) * row + c * 8);
-        }
-      }
+      for (int u = 0; u < kU; ++u)
+        if (t + u * groups < t1)
+          x[u] = ld_act_v4(src + static_cast<int64_t>(rows_s[t + u * groups - t0]) * row + c * 8);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int tt = t + u * groups;
-        if (tt < t1) {
-          *reinterpret_cast<uint4 *>(to + static_cast<int64_t>(tt - pi * a.page) * a.D) = x[u];
+      for (int u = 0; u < kU; ++u)
+        if (t + u * groups < t1) {
+          *reinterpret_cast<uint4 *>(to + static_cast<int64_t>(t + u * groups) * a.D) = x[u];
           if (full) fold(x[u]);
         }
-      }
     }
     if (full) {
       for (int t = pi * a.page + g; t < t0; t += groups)  // rows that were there before
-        fold(ld_act_v4(to + static_cast<int64_t>(t - pi * a.page) * a.D));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        bounds[(g * 2 + 0) * row + c * 8 + i] = nan ? -INFINITY : lo[i];
-        bounds[(g * 2 + 1) * row + c * 8 + i] = nan ? INFINITY : hi[i];
-      }
+        fold(ld_act_v4(to + static_cast<int64_t>(t) * a.D));
+      *reinterpret_cast<uint4 *>(bounds + (g * 2 + 0) * row + c * 8) = *reinterpret_cast<const uint4 *>(lo);
+      *reinterpret_cast<uint4 *>(bounds + (g * 2 + 1) * row + c * 8) = *reinterpret_cast<const uint4 *>(hi);
     }
   }
   if (!full) return;
@@ -304,6 +296,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_write_kernel(AppendArgs
   const int lane = threadIdx.x & 31;
   for (int h = threadIdx.x >> 5; h < a.Hkv; h += kAppendThreads / 32) {
     float lo[4], hi[4], top = 0.f;
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = i * 32 + lane;
@@ -311,13 +304,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_write_kernel(AppendArgs
       hi[i] = -INFINITY;
       if (d < a.D) {
         for (int q = 0; q < groups; ++q) {
-          lo[i] = fminf(lo[i], bounds[(q * 2 + 0) * row + h * a.D + d]);
-          hi[i] = fmaxf(hi[i], bounds[(q * 2 + 1) * row + h * a.D + d]);
+          const float l = bf16_bits_to_float(bounds[(q * 2 + 0) * row + h * a.D + d]);
+          const float u = bf16_bits_to_float(bounds[(q * 2 + 1) * row + h * a.D + d]);
+          nan |= l != l;
+          lo[i] = fminf(lo[i], l);
+          hi[i] = fmaxf(hi[i], u);
         }
         top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
       }
     }
-    top = warp_max(top);
+    top = warp_max(nan ? INFINITY : top);
     const float scale = __fdiv_rn(top, 127.f);
     const bool fine = top < INFINITY;
     const int64_t at = (static_cast<int64_t>(layer) * a.P + p) * a.Hkv + h;
@@ -346,6 +342,8 @@ struct ForkArgs {
   int *fresh;          // workspace [S]: the page a slot's partial page is copied to, or -1
   int *from;           // workspace [S]: the old slot, or -1
   int *list;           // workspace [S]: free pages
+  int4 *copies;        // workspace [S]: {old page, new page, rows} of the partial pages to copy
+  int *count;          // workspace [1]
   int64_t layer_stride;
   int layers, S, Hkv, D, page, P, M;
 };
@@ -396,10 +394,18 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
       a.from[s] = -1;
       atomicAdd(&refused, 1);
     }
+    if (rank >= 0 && !off) {
+      const int len = length[src[s]], p = ld_act_i32(a.table + static_cast<int64_t>(src[s]) * a.M + len / a.page);
+      // a table entry that is no page of the pool: nothing to copy
+      a.copies[rank] = make_int4(p, a.list[rank], p >= 0 && p < a.P ? len % a.page : 0, 0);
+    }
     a.lens_out[s] = src[s] >= 0 && !off ? length[src[s]] : 0;
   }
   __syncthreads();
-  if (threadIdx.x == 0) a.status[0] = refused;
+  if (threadIdx.x == 0) {
+    a.status[0] = refused;
+    a.count[0] = got;
+  }
 }
 
 constexpr int kCopyThreads = 256;
@@ -419,39 +425,50 @@ __device__ __forceinline__ void copy_block(const uint8_t *src, uint8_t *dst, int
   }
 }
 
-// Grid (S, 1 + 2 * layers, head groups): y 0 writes the slot's row and its reference
-// counts, y > 0 copies the valid rows of the slot's partial page in one layer of K or V.
+// Writes the new table and the reference counts, then copies the valid rows of the partial
+// pages: a warp per (copy, layer, K or V, head), rows * D contiguous values, 8 accesses of
+// 16 bytes in flight per lane. (A CTA per such item measured 85 us against 29 for 60 copies
+// in 16 layers and 8 heads, 122 MB moved: most CTAs had little or nothing to do.)
 __global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(ForkArgs a) {
-  const int s = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  const int r = ld_act_i32(a.from + s), fresh = ld_act_i32(a.fresh + s);
-  const int len = ld_act_i32(a.lens_out + s);
-  const int tail = len / a.page;  // place of the partial page
-  if (blockIdx.y == 0) {
+  const int lane = threadIdx.x & 31;
+  const int warp = blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5), warps = gridDim.x * (kCopyThreads / 32);
+  const int per = (a.M + 31) / 32;  // a warp takes 32 entries of one row
+  for (int64_t it = warp; it < static_cast<int64_t>(a.S) * per; it += warps) {
+    const int s = static_cast<int>(it / per), at = static_cast<int>(it % per) * 32 + lane;
+    const int r = ld_act_i32(a.from + s), fresh = ld_act_i32(a.fresh + s), len = ld_act_i32(a.lens_out + s);
+    if (at >= a.M) continue;
     const int pages = (len + a.page - 1) / a.page;
-    for (int at = blockIdx.z * kCopyThreads + threadIdx.x; at < a.M; at += gridDim.z * kCopyThreads) {
-      const int old = ld_act_i32(a.table + static_cast<int64_t>(s) * a.M + at);
-      int now = -1;
-      if (at < pages) now = at == tail && fresh >= 0 ? fresh : ld_act_i32(a.table + static_cast<int64_t>(r) * a.M + at);
-      a.table_out[static_cast<int64_t>(s) * a.M + at] = now;
-      if (old != now) {
-        if (old >= 0 && old < a.P) atomicSub(a.refs_out + old, 1);
-        if (now >= 0 && now < a.P) atomicAdd(a.refs_out + now, 1);
-      }
+    const int old = ld_act_i32(a.table + static_cast<int64_t>(s) * a.M + at);
+    int now = -1;
+    if (at < pages)
+      now = at == len / a.page && fresh >= 0 ? fresh : ld_act_i32(a.table + static_cast<int64_t>(r) * a.M + at);
+    a.table_out[static_cast<int64_t>(s) * a.M + at] = now;
+    if (old != now) {
+      if (old >= 0 && old < a.P) atomicSub(a.refs_out + old, 1);
+      if (now >= 0 && now < a.P) atomicAdd(a.refs_out + now, 1);
     }
-    return;
   }
-  if (fresh < 0) return;
-  const int p = ld_act_i32(a.table + static_cast<int64_t>(r) * a.M + tail);
-  if (p < 0 || p >= a.P) return;
-  const int plane = blockIdx.y - 1;
-  uint16_t *pool = ((plane & 1) ? a.v : a.k) + (plane >> 1) * a.layer_stride;
-  const int rows = len % a.page;
-  for (int h = blockIdx.z; h < a.Hkv; h += gridDim.z)
-    copy_block(reinterpret_cast<const uint8_t *>(pool + (static_cast<int64_t>(p) * a.Hkv + h) * a.page * a.D),
-               reinterpret_cast<uint8_t *>(pool + (static_cast<int64_t>(fresh) * a.Hkv + h) * a.page * a.D),
-               rows * a.D * 2);
+  const int planes = 2 * a.layers * a.Hkv;
+  const int64_t items = static_cast<int64_t>(ld_act_i32(a.count)) * planes;
+  for (int64_t it = warp; it < items; it += warps) {
+    const int4 c = *reinterpret_cast<const int4 *>(a.copies + it / planes);
+    const int plane = static_cast<int>(it % planes), h = plane % a.Hkv, lv = plane / a.Hkv;
+    uint16_t *pool = ((lv & 1) ? a.v : a.k) + (lv >> 1) * a.layer_stride;
+    const uint4 *from = reinterpret_cast<const uint4 *>(pool + (static_cast<int64_t>(c.x) * a.Hkv + h) * a.page * a.D);
+    uint4 *to = reinterpret_cast<uint4 *>(pool + (static_cast<int64_t>(c.y) * a.Hkv + h) * a.page * a.D);
+    const int n = c.z * a.D / 8;
+    for (int i = lane; i < n; i += 8 * 32) {
+      uint4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u * 32 < n) x[u] = ld_act_v4(from + i + u * 32);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u * 32 < n) to[i + u * 32] = x[u];
+    }
+  }
 }
 
 // ---- compact --------------------------------------------------------------------------
@@ -600,18 +617,18 @@ extern "C" int iron_page_append(const iron_page_pool *c, const uint16_t *k_new, 
   const int touched = min((num_new + a.page - 2) / a.page + 1, a.M);
   const int vpr = a.Hkv * a.D / 8, width = vpr < kAppendThreads ? vpr : kAppendThreads;
   const int groups = kAppendThreads / width < 64 ? kAppendThreads / width : 64;
-  const size_t smem = a.codes ? static_cast<size_t>(groups) * 2 * a.Hkv * a.D * sizeof(float) : 0;
+  const size_t smem = a.codes ? static_cast<size_t>(groups) * 2 * a.Hkv * a.D * sizeof(uint16_t) : 0;
   if (smem > 200 * 1024) return IRON_ERR_UNSUPPORTED;
+  auto kern = a.codes ? append_write_kernel<true> : append_write_kernel<false>;
   if (smem > 48 * 1024) {
-    const int e = call_status(cudaFuncSetAttribute(append_write_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(smem)));
+    const int e = call_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     if (e != IRON_OK) return e;
   }
-  return launch(append_write_kernel, dim3(touched, a.S, 2 * a.layers), dim3(kAppendThreads), smem, s, true, a);
+  return launch(kern, dim3(touched, a.S, 2 * a.layers), dim3(kAppendThreads), smem, s, true, a);
 }
 
 extern "C" size_t iron_page_fork_workspace_bytes(int slots) {
-  return slots > 0 ? static_cast<size_t>(slots) * 3 * sizeof(int) : 0;
+  return slots > 0 ? static_cast<size_t>(slots) * 7 * sizeof(int) + 16 : 0;
 }
 
 extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, int32_t *page_table_out,
@@ -621,6 +638,7 @@ extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, in
   if (chk != IRON_OK) return chk;
   if (!source || !c->lens || !page_table_out || !lens_out || !refs_out || !status || !workspace) return IRON_ERR_NULL;
   if (workspace_bytes < iron_page_fork_workspace_bytes(c->slots)) return IRON_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return IRON_ERR_ALIGN;
   const size_t tb = static_cast<size_t>(c->slots) * c->max_pages * sizeof(int), rb = c->num_pages * sizeof(int);
   // rows are gathered from the old table while the new one is written
   if (overlap(c->page_table, tb, page_table_out, tb) || overlap(c->refs, rb, refs_out, rb)) return IRON_ERR_ARG;
@@ -635,9 +653,11 @@ extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, in
   a.lens_out = lens_out;
   a.refs_out = refs_out;
   a.status = status;
-  a.fresh = static_cast<int *>(workspace);
+  a.copies = static_cast<int4 *>(workspace);
+  a.fresh = reinterpret_cast<int *>(a.copies + c->slots);
   a.from = a.fresh + c->slots;
   a.list = a.from + c->slots;
+  a.count = a.list + c->slots;
   a.layers = c->layers;
   a.S = c->slots;
   a.Hkv = c->kv_heads;
@@ -650,7 +670,7 @@ extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, in
   const int copiers = min(64, (a.P + kPlanThreads - 1) / kPlanThreads);
   int st = launch(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), 0, s, (flags & IRON_FLAG_PDL) != 0, a);
   if (st != IRON_OK) return st;
-  return launch(fork_copy_kernel, dim3(a.S, 1 + 2 * a.layers, a.Hkv < 8 ? a.Hkv : 8), dim3(kCopyThreads), 0, s, true, a);
+  return launch(fork_copy_kernel, dim3(sm_count() * 8), dim3(kCopyThreads), 0, s, true, a);
 }
 
 extern "C" size_t iron_page_compact_workspace_bytes(int num_pages) {

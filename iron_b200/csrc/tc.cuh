@@ -220,6 +220,20 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr, uint32_t
   return d;
 }
 
+// True in one lane of a converged warp, always the same one (commits track the issuing
+// thread's operations). The branch on elect.sync tells the compiler that a single thread
+// runs: in a branch on a lane number it issues every tcgen05.mma through a loop over the
+// lanes that could be active, about 94 cycles each (B200).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]: A's bf16 pairs lie in TMEM columns, K-major.
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {

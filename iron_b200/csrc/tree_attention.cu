@@ -16,6 +16,9 @@ constexpr int kTRows = 16;     // rows per unit
 constexpr int kTTile = 64;     // tokens per tile: 16 per warp
 constexpr int kTWarps = 4;
 constexpr int kTCtasPerSm = 4;
+struct TreeCut {
+  static constexpr int kTile = kTTile, kUnitCost = 1;
+};
 
 template <int D>
 __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(TreeArgs a) {
@@ -25,25 +28,25 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
   __shared__ __align__(16) uint8_t smem[kVBytes > kOBytes ? kVBytes : kOBytes];  // V tiles, then the merge
   __shared__ float red_m[kTWarps][kTRows], red_l[kTWarps][kTRows];
   __shared__ int pref[kTMaxBatch + 1], warp_sums[kTWarps];
-  __shared__ int parents[kTMaxNodes];
-  __shared__ uint32_t paths[kTRows][kTMaxNodes / 32];
+  __shared__ TreePaths tree;
+  __shared__ __align__(16) uint32_t paths[kTRows][kTMaxNodes / 32];
   __shared__ uint32_t usable[kTMaxNodes / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
   uint16_t *vs = reinterpret_cast<uint16_t *>(smem) + warp * 16 * Attn::kVStride;
   float (*red_o)[kTRows][D] = reinterpret_cast<float (*)[kTRows][D]>(smem);
   pdl_launch_dependents();
   pdl_wait();
-  tile_prefix<32 * kTWarps, kTTile>(a, pref, warp_sums);
+  cost_prefix<TreeCut, 32 * kTWarps>(a, pref, warp_sums);
   const int g = a.Hq / a.Hkv;
   const int64_t total = static_cast<int64_t>(pref[a.B]) * a.Hkv * a.groups;
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));  // none is empty
   if (static_cast<int>(blockIdx.x) >= pieces) return;
-  int64_t w = piece_start(total, blockIdx.x, pieces);
+  const int64_t w = piece_start(total, blockIdx.x, pieces);
   const int64_t w_end = piece_start(total, blockIdx.x + 1, pieces);
   const int page = 1 << a.page_shift;
 
-  while (w < w_end) {
-    const Segment sg = find_segment(a, pref, w, w_end);
+  for (Segment sg = next_segment<TreeCut>(a, pref, w, w_end); sg.count > 0;
+       sg = next_segment<TreeCut>(a, pref, sg.next, w_end)) {
     const int b = sg.b, h = sg.h, row0 = sg.group * kTRows, first = sg.first, count = sg.count;
     const int len = cached_len(a, b), ctiles = (len + kTTile - 1) / kTTile;
     const int *table = a.table + static_cast<int64_t>(b) * a.M;
@@ -55,22 +58,17 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
     at.load_q(r_lo < rows ? qb + r_lo / g * a.qs[1] + (h * g + r_lo % g) * a.qs[2] : nullptr,
               r_hi < rows ? qb + r_hi / g * a.qs[1] + (h * g + r_hi % g) * a.qs[2] : nullptr);
     if (first + count > ctiles) {  // the tree's nodes are part of this piece: their paths
-      for (int i = threadIdx.x; i < kTMaxNodes; i += 32 * kTWarps)
-        parents[i] = i < a.N ? ld_act_i32(a.parents + static_cast<int64_t>(b) * a.N + i) : -2;
-      __syncthreads();
-      if (threadIdx.x < kTMaxNodes) {
-        uint32_t bits[kTMaxNodes / 32];
-        const int i = threadIdx.x;
-        const bool used = i < a.N && tree_path(parents, i, bits);
-        const unsigned all = __ballot_sync(0xffffffffu, used);
-        if (lane == 0) usable[warp] = all;
-      }
-      if (threadIdx.x < kTRows) {
-        uint32_t bits[kTMaxNodes / 32] = {};
-        const int i = (row0 + threadIdx.x) / g;
-        if (i < a.N) tree_path(parents, i, bits);
+      if (warp == 0) {
+        tree_paths(tree, a.parents + static_cast<int64_t>(b) * a.N, a.N);
 #pragma unroll
-        for (int q = 0; q < kTMaxNodes / 32; ++q) paths[threadIdx.x][q] = bits[q];
+        for (int k = 0; k < kTMaxNodes / 32; ++k) {
+          const unsigned all = __ballot_sync(0xffffffffu, tree.up[k * 32 + lane] == -1);
+          if (lane == 0) usable[k] = all;
+        }
+        if (lane < kTRows) {
+          const int i = (row0 + lane) / g;
+          *reinterpret_cast<uint4 *>(paths[lane]) = i < a.N ? tree.bits[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
       }
       __syncthreads();
     }
@@ -141,7 +139,7 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
     __syncthreads();
     const bool whole = count == sg.tiles;
     const bool has_tree = first + count > ctiles;
-    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * kTRows * (2 + D);
+    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * kTRows * (2 + D);  // O, then (m, l)
     for (int idx = threadIdx.x; idx < kTRows * D; idx += 32 * kTWarps) {
       const int r = idx / D, d = idx % D;
       float M = -INFINITY, L = 0.f, O = 0.f;
@@ -163,48 +161,68 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
               float_to_bf16_bits(dead ? 0.f : normalised(O, L));
       } else {
         if (d == 0) {
-          part[r * (2 + D)] = M;
-          part[r * (2 + D) + 1] = dead ? -1.f : L;  // -1: the join writes zeros
+          part[kTRows * D + 2 * r] = M;
+          part[kTRows * D + 2 * r + 1] = dead ? -1.f : L;  // -1: the join writes zeros
         }
-        part[r * (2 + D) + 2 + d] = O;
+        part[r * D + d] = O;
       }
     }
     __syncthreads();  // shared memory is used again
-    w += count;
   }
 }
 
-// Joins the partials of one unit, in the order of its tiles. Units that one piece held
-// whole have nothing to join.
+// Joins the partials of one unit, in the order of its tiles; a thread owns 4 values of a
+// row. Units that one piece held whole have nothing to join. kJoin pieces are loaded at a
+// time, so a unit of many pieces costs a memory round trip per kJoin of them.
+constexpr int kJoin = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(kTRows *D / 4) tree_join_kernel(TreeArgs a, int ctas) {
   pdl_launch_dependents();
   pdl_wait();
   const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
   const int b = blockIdx.x / per, unit = blockIdx.x % per;
-  const UnitSpan sp = find_span<128, kTTile>(a, b, unit, ctas);
-  const int c0 = sp.c0, c1 = sp.c1;
-  if (c0 == c1) return;
-  const int h = unit / a.groups, row0 = unit % a.groups * kTRows, rows = a.N * g;
-  for (int idx = threadIdx.x; idx < kTRows * D; idx += 128) {
-    const int r = idx / D, d = idx % D, rr = row0 + r;
-    if (rr >= rows) break;
-    auto part = [&](int c) { return a.ws + ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * kTRows + r) * (2 + D); };
-    float M = -INFINITY;
-    bool dead = false;
-    for (int c = c0; c <= c1; ++c) {
-      M = fmaxf(M, ld_act_f32(part(c)));
-      dead |= ld_act_f32(part(c) + 1) < 0.f;
+  const UnitSpan sp = find_span<TreeCut, kTRows * D / 4>(a, b, unit, ctas);
+  if (sp.c0 == sp.c1) return;
+  const int h = unit / a.groups, r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const int row = unit % a.groups * kTRows + r;
+  if (row >= a.N * g) return;
+  float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+  bool dead = false;
+  for (int c = sp.c0; c <= sp.c1; c += kJoin) {
+    float2 ml[kJoin];
+    float4 o[kJoin];
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const bool in = c + i <= sp.c1;
+      const float *part = a.ws + (static_cast<int64_t>(in ? c + i : sp.c0) * 2 + (c + i == sp.c0 || !in ? 1 : 0)) * kTRows * (2 + D);
+      ml[i] = __ldcg(reinterpret_cast<const float2 *>(part + kTRows * D + 2 * r));
+      o[i] = __ldcg(reinterpret_cast<const float4 *>(part + r * D + d));
+      if (!in) ml[i] = make_float2(-INFINITY, 0.f), o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float L = 0.f, O = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const float f = rescale(ld_act_f32(part(c)), M);
-      L += ld_act_f32(part(c) + 1) * f;
-      O += ld_act_f32(part(c) + 2 + d) * f;
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].x);
+    const float f0 = rescale(M, top);
+    M = top;
+    L *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) O[e] *= f0;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const float f = rescale(ml[i].x, M);
+      dead |= ml[i].y < 0.f;
+      L += ml[i].y * f;
+      O[0] += o[i].x * f;
+      O[1] += o[i].y * f;
+      O[2] += o[i].z * f;
+      O[3] += o[i].w * f;
     }
-    a.out[b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d] =
-        float_to_bf16_bits(dead ? 0.f : normalised(O, L));
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
+  *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d) =
+      make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
 }
 
 }  // namespace iron
@@ -244,7 +262,8 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   if (c->layers != 1 || num_nodes <= 0 || num_heads <= 0 || num_heads % c->kv_heads) return IRON_ERR_SHAPE;
   const int g = num_heads / c->kv_heads;
   if (num_nodes > kTMaxNodes || g > 16 || c->slots > kTMaxBatch) return IRON_ERR_UNSUPPORTED;
-  if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new)) return IRON_ERR_ALIGN;
+  if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(out) || !aligned16(workspace))
+    return IRON_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8 || kv_strides[i] % 8 || out_strides[i] % 8) return IRON_ERR_ALIGN;
   if (workspace_bytes < iron_tree_attn_workspace_bytes(c->slots, num_nodes, num_heads, c->kv_heads, c->head_dim))
@@ -280,6 +299,6 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   const int pieces = tree_pieces();
   int st = launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps), 0, s, pdl, a);
   if (st != IRON_OK) return st;
-  return launch(wide ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv * a.groups), dim3(128), 0, s,
-                true, a, pieces);
+  return launch(wide ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv * a.groups),
+                dim3(wide ? kTRows * 32 : kTRows * 16), 0, s, true, a, pieces);
 }

@@ -35,22 +35,74 @@ __device__ unsigned g_tree_status;  // 0 = ok, else the first failing role's cod
 namespace treetc {
 
 constexpr int kTile = 128;
-constexpr int kThreads = 384;  // three warpgroups; warps 10 and 11 idle
+constexpr int kThreads = 384;  // three warpgroups
 // registers: 384 x 168 at launch = 2 x 128 x 216 (a row of S is 128 of them) + 128 x 72
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(kThreads * 168 == 256 * kSoftmaxRegs + 128 * kOtherRegs, "the split must not exceed the launch's registers");
+// a unit's start and end take as long as about 3 tiles (B200: 5 us against 1.1 to 2.6)
+struct Cut {
+  static constexpr int kTile = treetc::kTile, kUnitCost = 3;
+};
 constexpr int kMasks = 8;  // tiles' masks in flight: stages + 2 at least
-constexpr uint64_t kDeadline = 2000000000ull;  // per wait, ns
+
+// Bounded wait for a barrier phase: false after 2 s. The clock is read every 256 polls
+// only, which waits of the usual length never reach.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+  uint64_t start = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255u) == 0u) {
+      const uint64_t now = tc::globaltimer_ns();
+      if (start == 0) start = now;
+      else if (now - start > 2000000000ull) return false;
+    }
+  }
+}
 
 template <int D>
 struct Cfg {
   static constexpr int kStages = D == 64 ? 4 : 2;
+  // tables of paths in flight: preparing tile i means that tile i - kStages is done with
+  static constexpr int kTrees = kStages + 3;
   static constexpr int kPanels = D / 64;
   static constexpr uint32_t kPanel = kTile * 128;          // 128 rows x 64 bf16
   static constexpr uint32_t kOperand = kPanels * kPanel;   // Q tile, K tile or V tile
   static constexpr uint32_t kSmem = 1024 + 2 * kOperand + 2 * kStages * kOperand;
-  static constexpr int kPart = kTile * D + 2 * kTile;      // floats of one stream's partial: O, then (m, l)
+  static constexpr int kPart = kTile * D + 2 * kTile;      // floats of one stream's partial: O [D][128], then (m, l)
 };
+
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 struct Bars {  // mbarrier addresses
   uint32_t base;
@@ -60,12 +112,15 @@ struct Bars {  // mbarrier addresses
   template <int S> __device__ uint32_t vempty(int i) const { return base + 8 * (3 * S + i); }
   template <int S> __device__ uint32_t sfull(int i) const { return base + 8 * (4 * S + i); }
   template <int S> __device__ uint32_t pfull(int i) const { return base + 8 * (4 * S + 2 + i); }
-  template <int S> __device__ uint32_t ofull(int i) const { return base + 8 * (4 * S + 4 + i); }
-  template <int S> __device__ uint32_t qfull(int i) const { return base + 8 * (4 * S + 6 + i); }
-  template <int S> __device__ uint32_t odd() const { return base + 8 * (4 * S + 8); }
-  template <int S> __device__ uint32_t drain() const { return base + 8 * (4 * S + 9); }
-  template <int S> __device__ uint32_t other() const { return base + 8 * (4 * S + 10); }
-  template <int S> __device__ uint32_t joined() const { return base + 8 * (4 * S + 11); }
+  template <int S> __device__ uint32_t plast(int i) const { return base + 8 * (4 * S + 4 + i); }
+  template <int S> __device__ uint32_t ofull(int i) const { return base + 8 * (4 * S + 6 + i); }
+  template <int S> __device__ uint32_t qfull(int i) const { return base + 8 * (4 * S + 8 + i); }
+  template <int S> __device__ uint32_t vready(int i) const { return base + 8 * (4 * S + 14 + kMasks + i); }
+  template <int S> __device__ uint32_t paths(int i) const { return base + 8 * (5 * S + 14 + kMasks + i); }
+  template <int S> __device__ uint32_t drain() const { return base + 8 * (4 * S + 11); }
+  template <int S> __device__ uint32_t other() const { return base + 8 * (4 * S + 12); }
+  template <int S> __device__ uint32_t joined() const { return base + 8 * (4 * S + 13); }
+  template <int S> __device__ uint32_t mask(int i) const { return base + 8 * (4 * S + 14 + i); }
 };
 
 struct Maps {
@@ -92,11 +147,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
   using C = Cfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_store[4 * S + 12];
+  __shared__ __align__(8) uint64_t bar_store[5 * S + 14 + kMasks + C::kTrees];
   __shared__ uint32_t tmem_slot;
   __shared__ int pref[kTMaxBatch + 1], warp_sums[kThreads / 32];
-  __shared__ uint32_t masks[kMasks][4];
-  __shared__ int parents_s[8][kTMaxNodes];  // per softmax warp
+  __shared__ __align__(16) uint32_t masks[kMasks][4];
+  __shared__ TreePaths trees[C::kTrees];
   __shared__ float2 other_ml[kTile];        // (m, l) of stream 1, for the join of both streams
   __shared__ int odd_flag;                  // V of the tree held values that are not finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -107,7 +162,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
 
   pdl_launch_dependents();
   pdl_wait();
-  tile_prefix<kThreads, kTile>(a, pref, warp_sums);
+  cost_prefix<Cut, kThreads>(a, pref, warp_sums);
   const int64_t total = static_cast<int64_t>(pref[a.B]) * a.Hkv * a.groups;
   const int pieces = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));  // none is empty
   if (static_cast<int>(blockIdx.x) >= pieces) return;
@@ -118,11 +173,14 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init_u32(bars.sfull<S>(i), 1);
       tc::mbar_init_u32(bars.pfull<S>(i), 4);
+      tc::mbar_init_u32(bars.plast<S>(i), 4);
       tc::mbar_init_u32(bars.ofull<S>(i), 1);
       tc::mbar_init_u32(bars.qfull<S>(i), 4);
     }
-    tc::mbar_init_u32(bars.odd<S>(), 4);
+    for (int i = 0; i < S; ++i) tc::mbar_init_u32(bars.vready<S>(i), 2);
+    for (int i = 0; i < C::kTrees; ++i) tc::mbar_init_u32(bars.paths<S>(i), 1);
     tc::mbar_init_u32(bars.drain<S>(), 1);
+    for (int i = 0; i < kMasks; ++i) tc::mbar_init_u32(bars.mask<S>(i), 1);
     tc::mbar_init_u32(bars.other<S>(), 4);
     tc::mbar_init_u32(bars.joined<S>(), 4);
     odd_flag = 0;
@@ -146,8 +204,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     const int page = 1 << a.page_shift, ppt = kTile >> a.page_shift;  // pages per tile
     bool ok = true;
     int it = 0;
-    for (int64_t w = w_begin; w < w_end && ok;) {
-      const Segment sg = find_segment(a, pref, w, w_end);
+    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
       const int len = cached_len(a, sg.b), ctiles = (len + kTile - 1) / kTile;
       const int *table = a.table + static_cast<int64_t>(sg.b) * a.M;
       // 32 table entries at a time, the next ones requested while these are used
@@ -179,11 +237,14 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, n > 0));
         const uint32_t bytes = tree ? C::kOperand : boxes * page * D * 2;
         const uint32_t parity = ((it / S) & 1) ^ 1;
-        ok = __all_sync(0xffffffffu, tc::wait_until(bars.kempty<S>(s), parity, kDeadline));
+        ok = __all_sync(0xffffffffu, wait_phase(bars.kempty<S>(s), parity));
         if (!ok) break;
         if (lane < 4) masks[it % kMasks][lane] = bits;
         __syncwarp();
-        if (lane == 0) tc::expect_tx(bars.kfull<S>(s), bytes);
+        if (lane == 0) {
+          tc::arrive(bars.mask<S>(it % kMasks));
+          tc::expect_tx(bars.kfull<S>(s), bytes);
+        }
         __syncwarp();
         auto load = [&](const CUtensorMap *pages, const CUtensorMap *fresh, uint32_t dst, uint32_t bar) {
           if (tree) {
@@ -195,47 +256,47 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           }
         };
         load(&maps.k, &maps.k_new, k0 + s * C::kOperand, bars.kfull<S>(s));
-        ok = __all_sync(0xffffffffu, tc::wait_until(bars.vempty<S>(s), parity, kDeadline));
+        ok = __all_sync(0xffffffffu, wait_phase(bars.vempty<S>(s), parity));
         if (!ok) {
           // this tile's K is on its way already: let it land
-          tc::wait_until(bars.kfull<S>(s), (it / S) & 1, 100000000ull);
+          wait_phase(bars.kfull<S>(s), (it / S) & 1);
           break;
         }
         if (lane == 0) tc::expect_tx(bars.vfull<S>(s), bytes);
         __syncwarp();
         load(&maps.v, &maps.v_new, v0 + s * C::kOperand, bars.vfull<S>(s));
       }
-      w += sg.count;
     }
     if (!ok) {
       if (lane == 0) atomicCAS(&g_tree_status, 0u, 1u);
       // copies in flight land before the CTA's shared memory goes away
       for (int j = max(0, it - S); j < it; ++j) {
-        tc::wait_until(bars.kfull<S>(j % S), (j / S) & 1, 100000000ull);
-        tc::wait_until(bars.vfull<S>(j % S), (j / S) & 1, 100000000ull);
+        wait_phase(bars.kfull<S>(j % S), (j / S) & 1);
+        wait_phase(bars.vfull<S>(j % S), (j / S) & 1);
       }
     }
     } else if (warp == 8) {
-    // ---- MMAs, one thread ----
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, kTile);
-      constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
-      bool ok = true;
-      int it0 = 0;
-      uint32_t pc[2] = {0, 0}, qc[2] = {0, 0};
-      for (int64_t w = w_begin; w < w_end && ok;) {
-        const Segment sg = find_segment(a, pref, w, w_end);
-        const Streams st = streams_of(a, sg);
-        auto tile_of = [&](int s, int j) { return it0 + (st.both ? j : 2 * j + s); };
-        auto scores = [&](int s, int j) {
-          const int it = tile_of(s, j), slot = it % S;
-          ok = ok && tc::wait_until(bars.kfull<S>(slot), (it / S) & 1, kDeadline);
-          if (!ok) return;
-          tc::fence_after_sync();
-          // a step of the start address is a step of the descriptor's low bits (16-byte units)
-          const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
-          const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand);
-#pragma unroll 1
+    // ---- MMAs: the warp stays converged, an elected lane issues ----
+    constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, kTile);
+    constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
+    bool ok = true;
+    int it0 = 0;
+    uint32_t pc[2] = {0, 0}, qc[2] = {0, 0};
+    auto ready = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_phase(bar, parity)) != 0; };
+    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
+      const Streams st = streams_of(a, sg);
+      auto tile_of = [&](int s, int j) { return it0 + (st.both ? j : 2 * j + s); };
+      auto scores = [&](int s, int j) {
+        const int it = tile_of(s, j), slot = it % S;
+        ok = ready(bars.kfull<S>(slot), (it / S) & 1);
+        if (!ok) return;
+        tc::fence_after_sync();
+        // a step of the start address is a step of the descriptor's low bits (16-byte units)
+        const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
+        const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand);
+        if (tc::elect_one()) {
+#pragma unroll
           for (int c = 0; c < C::kPanels; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
@@ -243,43 +304,116 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
                            c > 0 || kk > 0);
           tc::mma_commit(bars.sfull<S>(s));
           if (!st.both || s == 1) tc::mma_commit(bars.kempty<S>(slot));
-        };
-        auto values = [&](int s, int j) {
-          const int it = tile_of(s, j), slot = it % S;
-          ok = ok && tc::wait_until(bars.pfull<S>(s), pc[s]++ & 1, kDeadline) &&
-               tc::wait_until(bars.vfull<S>(slot), (it / S) & 1, kDeadline);
-          if (!ok) return;
-          tc::fence_after_sync();
-          const uint32_t p = tmem + s * 128, o = tmem + 256 + s * D;
-          const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand, C::kPanel);
-#pragma unroll 1
+        }
+        __syncwarp();
+      };
+      // in two halves of 64 tokens: the first runs while the second's softmax does
+      auto values = [&](int s, int j) {
+        const int it = tile_of(s, j), slot = it % S;
+        const uint32_t p = tmem + s * 128, o = tmem + 256 + s * D, parity = pc[s]++ & 1;
+        const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand, C::kPanel);
+        ok = ready(bars.vready<S>(slot), (it / S) & 1) && ready(bars.pfull<S>(s), parity);
+        if (!ok) return;
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+#pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
+            for (int kk = 0; kk < 4; ++kk)
               tc::mma_bf16_ts(o, p + part * 64 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || part > 0 || kk > 0);
+        }
+        __syncwarp();
+        ok = ready(bars.plast<S>(s), parity);
+        if (!ok) return;
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk)
+              tc::mma_bf16_ts(o, p + part * 64 + kk * 8, v + kk * (2048 >> 4), idesc_o, 1);
           if (!st.both || s == 1) tc::mma_commit(bars.vempty<S>(slot));
           if (j == st.n[s] - 1) tc::mma_commit(bars.ofull<S>(s));
-        };
+        }
+        __syncwarp();
+      };
+      for (int s = 0; s < 2; ++s)
+        if (st.n[s] > 0 && ok) {
+          ok = ready(bars.qfull<S>(s), qc[s]++ & 1);
+          if (ok) scores(s, 0);
+        }
+      for (int j = 0; j < st.n[0] && ok; ++j)
         for (int s = 0; s < 2; ++s)
-          if (st.n[s] > 0 && ok) {
-            ok = tc::wait_until(bars.qfull<S>(s), qc[s]++ & 1, kDeadline);
-            if (ok) scores(s, 0);
+          if (j < st.n[s]) {
+            if (ok) values(s, j);
+            if (ok && j + 1 < st.n[s]) scores(s, j + 1);
           }
-        for (int j = 0; j < st.n[0] && ok; ++j)
-          for (int s = 0; s < 2; ++s)
-            if (j < st.n[s]) {
-              if (ok) values(s, j);
-              if (ok && j + 1 < st.n[s]) scores(s, j + 1);
-            }
-        it0 += sg.count;
-        w += sg.count;
-      }
-      if (!ok) atomicCAS(&g_tree_status, 0u, 2u);
-      // every MMA issued is done before TMEM is freed
-      tc::mma_commit(bars.drain<S>());
-      tc::wait_until(bars.drain<S>(), 0, kDeadline);
+      it0 += sg.count;
     }
+    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
+    // every MMA issued is done before TMEM is freed
+    if (tc::elect_one()) tc::mma_commit(bars.drain<S>());
     __syncwarp();
+    wait_phase(bars.drain<S>(), 0);
+    __syncwarp();
+    } else {
+    // ---- preparation: warp 10 and 11 ----
+    bool ok = true;
+    int it = 0, trees_done = 0;
+    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
+      const int ctiles = (cached_len(a, sg.b) + kTile - 1) / kTile;
+      TreePaths &tree = trees[trees_done % C::kTrees];
+      if (sg.first + sg.count > ctiles) {
+        if (warp == 10) {
+          tree_paths(tree, a.parents + static_cast<int64_t>(sg.b) * a.N, a.N);
+          if (lane == 0) tc::arrive(bars.paths<S>(trees_done % C::kTrees));
+        } else {
+          ok = __all_sync(0xffffffffu, wait_phase(bars.paths<S>(trees_done % C::kTrees), (trees_done / C::kTrees) & 1));
+          if (!ok) break;
+        }
+        ++trees_done;
+      }
+      for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
+        const int slot = it % S;
+        ok = __all_sync(0xffffffffu, wait_phase(bars.vfull<S>(slot), (it / S) & 1));
+        if (!ok) break;
+        const bool nodes = i >= ctiles;
+        const uint4 valid = *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
+        if (nodes || (valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {
+          // rows of V that hold nothing are zeroed, and so are a node's values that are not
+          // finite (0 * inf is not 0; rows that see them get them added at the end)
+          bool odd = false;
+#pragma unroll 1
+          for (int r = (warp - 10) * 32 + lane; r < kTile; r += 64) {
+            const bool keep = nodes ? tree.up[r] == -1 : masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
+            if (keep && !nodes) continue;
+            uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              // lanes start at different pieces of their rows: no bank conflicts
+              uint4 *e = reinterpret_cast<uint4 *>(vrow + (c >> 3) * C::kPanel + (((c & 7) ^ (r & 7)) << 4));
+              uint4 y = keep ? *e : make_uint4(0, 0, 0, 0);
+              bool change = !keep;
+              if (keep) {
+                uint32_t *u = reinterpret_cast<uint32_t *>(&y);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u, change = odd = true;
+                  if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu, change = odd = true;
+                }
+              }
+              if (change) *e = y;
+            }
+          }
+          if (odd) atomicExch(&odd_flag, 1);
+          tc::fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) tc::arrive(bars.vready<S>(slot));
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 5u);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -288,13 +422,41 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
     uint8_t *qs = smem + s * C::kOperand;
-    int *parents = parents_s[warp];
     bool ok = true;
     int it0 = 0;
-    uint32_t sc = 0, oc = 0, fc = 0, jc = 0;
-    for (int64_t w = w_begin; w < w_end && ok;) {
-      const Segment sg = find_segment(a, pref, w, w_end);
-      const Streams st = streams_of(a, sg);
+    uint32_t sc = 0, oc = 0, jc = 0;
+    int trees_seen = 0;
+    // The stream's rows of Q into shared memory, swizzled as TMA would write them (16-byte
+    // piece c of row r at c ^ (r % 8)): 8 lanes per row and panel of 64. The first S of the
+    // segment may run as soon as they are there, while the segment before is still written out.
+    auto load_q = [&](const Segment &g_, const Streams &st) {
+      if (st.n[s] == 0) return;
+      const int own = g_.group * 256 + (st.both ? s * 128 : 0) + r;
+      const int64_t off = own < rows_all ? g_.b * a.qs[0] + own / g * a.qs[1] + (g_.h * g + own % g) * a.qs[2] : -1;
+      uint4 x[8 * C::kPanels];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, off, i * 4 + (lane >> 3));
+#pragma unroll
+        for (int c = 0; c < C::kPanels; ++c)
+          x[i * C::kPanels + c] = at >= 0 ? ld_act_v4(a.q + at + c * 64 + (lane & 7) * 8) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (warp & 3) * 32 + i * 4 + (lane >> 3);
+#pragma unroll
+        for (int c = 0; c < C::kPanels; ++c)
+          *reinterpret_cast<uint4 *>(qs + c * C::kPanel + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) =
+              x[i * C::kPanels + c];
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::arrive(bars.qfull<S>(s));
+    };
+    Segment sg = next_segment<Cut>(a, pref, w_begin, w_end);
+    Streams st = streams_of(a, sg);
+    if (sg.count > 0) load_q(sg, st);
+    while (sg.count > 0) {
       const int b = sg.b, h = sg.h, n = st.n[s];
       const int len = cached_len(a, b), ctiles = (len + kTile - 1) / kTile;
       const bool has_tree = sg.first + sg.count > ctiles;
@@ -302,94 +464,35 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       const bool live = row < rows_all;
       const int node = live ? row / g : 0, hq = h * g + (live ? row % g : 0);
       float m = -INFINITY, l = 0.f;
-      uint32_t path[4] = {0, 0, 0, 0};
-      if (n > 0) {
-        // the row of Q, swizzled as TMA would write it: 16-byte piece c of row r at c ^ (r % 8)
-        const uint16_t *q = a.q + b * a.qs[0] + node * a.qs[1] + hq * a.qs[2];
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = live ? ld_act_v4(q + c * 8) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(qs + (c >> 3) * C::kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
-        }
-        if (has_tree) {
-          for (int i = lane; i < kTMaxNodes; i += 32)
-            parents[i] = i < a.N ? ld_act_i32(a.parents + static_cast<int64_t>(b) * a.N + i) : -2;
-          __syncwarp();
-          if (live) tree_path(parents, node, path);
-        }
-        tc::fence_proxy_async_smem();
-        tc::fence_before_sync();  // the last segment's O has been read
-        __syncwarp();
-        if (lane == 0) tc::arrive(bars.qfull<S>(s));
-      }
+      uint4 path = make_uint4(0u, 0u, 0u, 0u);
       for (int j = 0; j < n; ++j) {
         const int i = sg.first + (st.both ? j : 2 * j + s), it = it0 + i - sg.first, slot = it % S;
-        ok = __all_sync(0xffffffffu, tc::wait_until(bars.sfull<S>(s), sc++ & 1, kDeadline) &&
-                                         tc::wait_until(bars.kfull<S>(slot), (it / S) & 1, kDeadline));
+        // (the masks have barriers of their own: K's may be a phase further by now)
+        ok = __all_sync(0xffffffffu, wait_phase(bars.sfull<S>(s), sc++ & 1) &&
+                                         wait_phase(bars.mask<S>(it % kMasks), (it / kMasks) & 1));
         if (!ok) break;
         tc::fence_after_sync();
         uint32_t x[128];
         tc::tmem_ld64(ts, x);
         tc::tmem_ld64(ts + 64, x + 64);
-        const bool tree = i >= ctiles;
-        uint32_t see[4];
-        bool all = true;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t valid = masks[it % kMasks][q];
-          see[q] = tree ? path[q] : valid;
-          all = all && valid == 0xffffffffu;
+        const bool nodes = i >= ctiles;
+        if (has_tree && j == n - 1) {  // the row's path, while its table is there
+          ok = __all_sync(0xffffffffu, wait_phase(bars.paths<S>(trees_seen % C::kTrees), (trees_seen / C::kTrees) & 1));
+          if (!ok) break;
+          if (live) path = trees[trees_seen % C::kTrees].bits[node];
         }
-        if (tree || !all) {  // the same for all threads
+        const uint4 valid = *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
+        if (nodes || (valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {  // the same for all threads
+          const uint32_t see[4] = {nodes ? path.x : valid.x, nodes ? path.y : valid.y, nodes ? path.z : valid.z,
+                                   nodes ? path.w : valid.w};
 #pragma unroll
           for (int t = 0; t < 128; ++t)
             if (!(see[t >> 5] >> (t & 31) & 1u)) x[t] = 0xff800000u;  // -inf
-          if (!st.both || s == 0) {
-            // row r of V: zero where the tile holds nothing, and where a node's value is not
-            // finite (0 * inf is not 0; rows that see it get it added at the end)
-            ok = __all_sync(0xffffffffu, tc::wait_until(bars.vfull<S>(slot), (it / S) & 1, kDeadline));
-            if (!ok) break;
-            bool keep;
-            if (tree) {
-              uint32_t unused[4];
-              keep = r < a.N && tree_path(parents, r, unused);
-            } else {
-              keep = masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
-            }
-            uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
-            bool odd = false;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              uint4 *e = reinterpret_cast<uint4 *>(vrow + (c >> 3) * C::kPanel + ((c & 7) << 4));
-              if (!keep) {
-                *e = make_uint4(0, 0, 0, 0);
-              } else if (tree) {
-                uint4 y = *e;
-                uint32_t *u = reinterpret_cast<uint32_t *>(&y);
-                bool change = false;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u, change = true;
-                  if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu, change = true;
-                }
-                if (change) {
-                  *e = y;
-                  odd = true;
-                }
-              }
-            }
-            if (odd) atomicExch(&odd_flag, 1);
-            tc::fence_proxy_async_smem();
-            if (tree && st.both) {
-              __syncwarp();
-              if (lane == 0) tc::arrive(bars.odd<S>());
-            }
-          }
         }
         // the row's maximum, its factor and the probabilities
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int t = 0; t < 128; ++t) mx[t & 3] = fmaxf(mx[t & 3], __uint_as_float(x[t]));
+        for (int t = 0; t < 128; t += 2) mx[(t >> 1) & 3] = max3(mx[(t >> 1) & 3], __uint_as_float(x[t]), __uint_as_float(x[t + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
         if (j == 0) {
           m = top;
@@ -426,32 +529,44 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           ref = 0.f;
           by = 1.f;
         }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), minus = pack2(-1.f, -1.f);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(x[32 * c + 2 * q]), by, -ref));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(x[32 * c + 2 * q + 1]), by, -ref));
-            sum[q & 1] += p0;
-            sum[2 + (q & 1)] += p1;
+            float p0, p1;
+            unpack2(fma2(pack2(__uint_as_float(x[32 * c + 2 * q]), __uint_as_float(x[32 * c + 2 * q + 1])), by2, ref2), p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+            const uint64_t p = pack2(p0, p1);
+            sum[q & 1] = add2(sum[q & 1], p);
             hi[q] = pack_bf16x2(p0, p1);
-            lo[q] = pack_bf16x2(p0 - bf16_lo(hi[q]), p1 - bf16_hi(hi[q]));
+            unpack2(fma2(pack2(bf16_lo(hi[q]), bf16_hi(hi[q])), minus, p), p0, p1);
+            lo[q] = pack_bf16x2(p0, p1);
           }
           tc::tmem_st16(ts + 16 * c, hi);
           tc::tmem_st16(ts + 64 + 16 * c, lo);
+          if (c & 1) {  // a half is there
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::arrive(c == 1 ? bars.pfull<S>(s) : bars.plast<S>(s));
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tc::tmem_st_wait();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::arrive(bars.pfull<S>(s));
+        float s0, s1;
+        unpack2(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
       }
       if (!ok) break;
+      trees_seen += has_tree;
+      const Segment next = next_segment<Cut>(a, pref, sg.next, w_end);
+      const Streams nst = streams_of(a, next);
+      if (next.count > 0) load_q(next, nst);  // every S of this stream is complete: Q may be replaced
       // ---- the segment's result ----
       const bool direct = sg.count == sg.tiles, join = !st.both && st.n[1] > 0;
-      if (n > 0) ok = __all_sync(0xffffffffu, tc::wait_until(bars.ofull<S>(s), oc++ & 1, kDeadline));
+      if (n > 0) ok = __all_sync(0xffffffffu, wait_phase(bars.ofull<S>(s), oc++ & 1));
       if (!ok) break;
       if (join && s == 1) {
         other_ml[r] = make_float2(m, l);
@@ -459,13 +574,13 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         __syncwarp();
         if (lane == 0) tc::arrive(bars.other<S>());
         // stream 0 reads this stream's O from TMEM before the next segment overwrites it
-        ok = __all_sync(0xffffffffu, tc::wait_until(bars.joined<S>(), jc++ & 1, kDeadline));
+        ok = __all_sync(0xffffffffu, wait_phase(bars.joined<S>(), jc++ & 1));
         if (!ok) break;
         tc::fence_after_sync();
       } else if (n > 0) {
         float f0 = 1.f, f1 = 0.f;
         if (join) {
-          ok = __all_sync(0xffffffffu, tc::wait_until(bars.other<S>(), jc++ & 1, kDeadline));
+          ok = __all_sync(0xffffffffu, wait_phase(bars.other<S>(), jc++ & 1));
           if (!ok) break;
           const float2 o = other_ml[r];
           const float M = fmaxf(m, o.x);
@@ -474,12 +589,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           l = l * f0 + o.y * f1;
           m = M;
         }
-        if (has_tree && st.both) {
-          ok = __all_sync(0xffffffffu, tc::wait_until(bars.odd<S>(), fc++ & 1, kDeadline));
-          if (!ok) break;
-        }
         tc::fence_after_sync();
-        const bool dead = has_tree && (path[0] | path[1] | path[2] | path[3]) == 0;
+        const bool dead = has_tree && (path.x | path.y | path.z | path.w) == 0;
         const bool odd = has_tree && *reinterpret_cast<volatile int *>(&odd_flag) != 0;
         const float inv = l == 0.f || dead ? 0.f : 1.f / l;
         uint16_t *dst = a.out + b * a.os[0] + node * a.os[1] + hq * a.os[2];
@@ -497,7 +608,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           }
           if (odd && live)
             for (int j = 0; j < a.N; ++j) {
-              if (!(path[j >> 5] >> (j & 31) & 1u)) continue;
+              const uint32_t word = j < 32 ? path.x : j < 64 ? path.y : j < 96 ? path.z : path.w;
+              if (!(word >> (j & 31) & 1u)) continue;
               const uint16_t *v = a.v_new + b * a.ks[0] + j * a.ks[1] + h * a.ks[2] + c;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
@@ -520,9 +632,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
                 *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(y[0], y[1], y[2], y[3]);
               }
           } else {
+            // column by column: the lanes of a warp write 128 contiguous bytes
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4 *>(part + r * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 32; ++e) part[(c + e) * kTile + r] = __uint_as_float(o[e]);
           }
         }
         if (!direct) {
@@ -536,7 +648,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         }
       }
       it0 += sg.count;
-      w += sg.count;
+      sg = next;
+      st = nst;
     }
     if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 3u + s);
   }
@@ -545,47 +658,68 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
   if (warp == 8) tc::tmem_free(tmem, 512);
 }
 
-// Joins the partials of 16 rows of one unit: 256 threads, D / 4 float4 columns x rows.
+// Joins the partials of 32 rows of one unit, in the order of its tiles: lane = row, a warp
+// per D / 8 dimensions, kJoin pieces loaded at a time.
 template <int D>
 __global__ void __launch_bounds__(256) tree_tc_join_kernel(TreeArgs a, int ctas) {
   using C = Cfg<D>;
+  constexpr int kDims = D / 8, kJoin = 32 / kDims;
   pdl_launch_dependents();
   pdl_wait();
   const int per = a.Hkv * a.groups, g = a.Hq / a.Hkv;
   const int b = blockIdx.x / per, unit = blockIdx.x % per, h = unit / a.groups, group = unit % a.groups;
-  const int rows = min(256, a.N * g - group * 256);
-  if (static_cast<int>(blockIdx.y) * 16 >= rows) return;
-  const UnitSpan sp = find_span<256, kTile>(a, b, unit, ctas);
+  const int rows = min(256, a.N * g - group * 256), first = blockIdx.y * 32;
+  if (first >= rows) return;
+  const UnitSpan sp = find_span<Cut, 256>(a, b, unit, ctas);
   if (sp.c0 == sp.c1) return;  // written by the piece that held it
-  for (int idx = threadIdx.x; idx < 16 * D / 4; idx += 256) {
-    const int ru = blockIdx.y * 16 + idx / (D / 4), d = idx % (D / 4) * 4;
-    if (ru >= rows) break;
-    const int r = ru % 128, s = ru / 128;
-    auto part = [&](int c) { return a.ws + ((static_cast<int64_t>(c) * 2 + (c == sp.c0 ? 1 : 0)) * 2 + s) * C::kPart; };
-    float M = -INFINITY;
-    bool dead = false;
-    for (int c = sp.c0; c <= sp.c1; ++c) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(c) + kTile * D + 2 * r));
-      M = fmaxf(M, ml.x);
-      dead |= ml.y < 0.f;
-    }
-    float L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = sp.c0; c <= sp.c1; ++c) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(c) + kTile * D + 2 * r));
-      const float4 o = __ldcg(reinterpret_cast<const float4 *>(part(c) + r * D + d));
-      const float f = rescale(ml.x, M);
-      L += ml.y * f;
-      O[0] += o.x * f;
-      O[1] += o.y * f;
-      O[2] += o.z * f;
-      O[3] += o.w * f;
-    }
+  const int ru = first + (threadIdx.x & 31), d0 = (threadIdx.x >> 5) * kDims;
+  const int r = ru % 128, s = ru / 128;
+  float M = -INFINITY, L = 0.f, O[kDims];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
-    const int row = group * 256 + ru;
-    *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d) =
-        make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
+  for (int e = 0; e < kDims; ++e) O[e] = 0.f;
+  bool dead = false;
+  for (int c = sp.c0; c <= sp.c1; c += kJoin) {
+    float2 ml[kJoin];
+    float o[kJoin][kDims];
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const bool in = c + i <= sp.c1;
+      const float *part = a.ws + ((static_cast<int64_t>(in ? c + i : sp.c0) * 2 + (c + i == sp.c0 || !in ? 1 : 0)) * 2 + s) * C::kPart;
+      ml[i] = __ldcg(reinterpret_cast<const float2 *>(part + kTile * D + 2 * r));
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) o[i][e] = __ldcg(part + (d0 + e) * kTile + r);
+      if (!in) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) o[i][e] = 0.f;
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].x);
+    const float f0 = rescale(M, top);
+    M = top;
+    L *= f0;
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) O[e] *= f0;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const float f = rescale(ml[i].x, M);
+      dead |= ml[i].y < 0.f;
+      L += ml[i].y * f;
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) O[e] += o[i][e] * f;
+    }
   }
+  if (ru >= rows) return;
+  const int row = group * 256 + ru;
+  uint16_t *dst = a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d0;
+#pragma unroll
+  for (int e = 0; e < kDims; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
+#pragma unroll
+  for (int e = 0; e < kDims; e += 8)
+    *reinterpret_cast<uint4 *>(dst + e) = make_uint4(pack_bf16x2(O[e], O[e + 1]), pack_bf16x2(O[e + 2], O[e + 3]),
+                                                     pack_bf16x2(O[e + 4], O[e + 5]), pack_bf16x2(O[e + 6], O[e + 7]));
 }
 
 static int make_map(CUtensorMap *m, const void *ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], int rows) {
@@ -623,7 +757,7 @@ static int launch_tc(TreeArgs a, bool pdl, cudaStream_t s) {
   st = launch(tree_tc_kernel<D>, dim3(ctas), dim3(kThreads), C::kSmem, s, pdl, maps, a);
   if (st != IRON_OK) return st;
   const int rows = a.N * (a.Hq / a.Hkv);
-  return launch(tree_tc_join_kernel<D>, dim3(a.B * a.Hkv * a.groups, ((rows < 256 ? rows : 256) + 15) / 16), dim3(256), 0, s,
+  return launch(tree_tc_join_kernel<D>, dim3(a.B * a.Hkv * a.groups, ((rows < 256 ? rows : 256) + 31) / 32), dim3(256), 0, s,
                 true, a, ctas);
 }
 

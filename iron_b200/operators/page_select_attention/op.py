@@ -26,7 +26,7 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, strides
+from ...common.paged import PagedOperator, address, strides
 from ...common.verify import Tolerance
 
 _I64x2 = ctypes.c_int64 * 2
@@ -72,7 +72,7 @@ class PageSelectAttention(PagedOperator):
             self.batch, self.num_heads, self.num_kv_heads, self.head_dim, self.max_pages, self.top_pages, self.page_size)
 
     def _launch(self, q, k_pages, v_pages, codes, scales, page_table, lens, out, selected, *, stream, flags=0):
-        p = _lib.dptr
+        p = address
         rows = (self.batch, self.num_heads, self.head_dim)
         ws, nbytes = self._workspace(stream)
         pool = _lib.PagePool(p(k_pages), p(v_pages), p(codes), p(scales), p(page_table), p(lens), None, 1, self.batch,

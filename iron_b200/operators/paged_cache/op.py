@@ -17,7 +17,7 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator
+from ...common.paged import PagedOperator, address
 
 
 @dataclass
@@ -52,8 +52,9 @@ class _PoolOperator(PagedOperator):
                 AIERuntimeArgSpec("inout", at, dtype=np.float32)]
 
     def _pool(self, k, v, table, lens, refs, codes=None, scales=None):
-        p = _lib.dptr
-        return _lib.PagePool(p(k), p(v), p(codes), p(scales), p(table), p(lens), p(refs), self.num_layers, self.slots,
+        p = address
+        return _lib.PagePool(p(k), p(v), codes if codes is None else p(codes), scales if scales is None else p(scales),
+                             p(table), lens if lens is None else p(lens), p(refs), self.num_layers, self.slots,
                              self.num_pages, self.max_pages, self.num_kv_heads, self.head_dim, self.page_size)
 
 
@@ -89,7 +90,7 @@ class PageAppend(_PoolOperator):
         return _lib.load().iron_page_append_workspace_bytes(self.slots, self.num_pages)
 
     def _launch(self, k_new, v_new, index, k, v, table, lens, refs, lens_out, status, *summary, stream, flags=0):
-        p = _lib.dptr
+        p = address
         ws, nbytes = self._workspace(stream)
         _lib.call("iron_page_append", ctypes.byref(self._pool(k, v, table, lens, refs, *summary)), p(k_new), p(v_new),
                   p(index), self.num_new, p(lens_out), p(status), ws, nbytes, flags, stream)
@@ -117,7 +118,7 @@ class PageFork(_PoolOperator):
         return _lib.load().iron_page_fork_workspace_bytes(self.slots)
 
     def _launch(self, source, table, lens, refs, k, v, table_out, lens_out, refs_out, status, *, stream, flags=0):
-        p = _lib.dptr
+        p = address
         ws, nbytes = self._workspace(stream)
         _lib.call("iron_page_fork", ctypes.byref(self._pool(k, v, table, lens, refs)), p(source), p(table_out),
                   p(lens_out), p(refs_out), p(status), ws, nbytes, flags, stream)
@@ -143,7 +144,7 @@ class PageCompact(_PoolOperator):
         return _lib.load().iron_page_compact_workspace_bytes(self.num_pages)
 
     def _launch(self, table, refs, k, v, table_out, refs_out, used, *summary, stream, flags=0):
-        p = _lib.dptr
+        p = address
         ws, nbytes = self._workspace(stream)
         _lib.call("iron_page_compact", ctypes.byref(self._pool(k, v, table, None, refs, *summary)), p(table_out),
                   p(refs_out), p(used), ws, nbytes, flags, stream)

@@ -27,7 +27,7 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, strides
+from ...common.paged import PagedOperator, address, strides
 from ...common.verify import Tolerance
 
 _I64x3 = ctypes.c_int64 * 3
@@ -73,7 +73,7 @@ class TreeAttention(PagedOperator):
                                                           self.num_kv_heads, self.head_dim)
 
     def _launch(self, q, k_new, v_new, k_pages, v_pages, page_table, lens, parents, out, *, stream, flags=0):
-        p = _lib.dptr
+        p = address
         new = (self.batch, self.num_nodes, self.num_kv_heads, self.head_dim)
         rows = (self.batch, self.num_nodes, self.num_heads, self.head_dim)
         ks = strides(k_new, new)
