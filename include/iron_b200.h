@@ -425,6 +425,8 @@ int iron_attn_prefill(const uint16_t *q, const uint16_t *k, const uint16_t *v, u
  *   refs     int32 [num_pages]: how many table rows hold the page (0: free).
  * head_dim 64 or 128; page_size 16, 32, 64 or 128; page * max_pages < 2^31; pools and
  * codes 16-byte aligned. Table entries outside [0, num_pages) are never followed.
+ * These entry points read nothing before they have waited for the stream's previous
+ * kernel, so they always launch the way IRON_FLAG_PDL asks for; the flag changes nothing.
  *
  * The summary of a full page, per kv head: lo, hi = the smallest and largest key per
  * dimension, scale = max |key| / 127, codes floor(lo / scale) and ceil(hi / scale) clamped
@@ -500,7 +502,7 @@ int iron_tree_attn(const iron_page_pool *pool, const uint16_t *q, const uint16_t
  * the order of summation. (a = 0 or not finite: all q8 = 0.) q, out bf16 [slots, Hq, D]
  * with element strides {batch, head} (2 int64 each, multiples of 8); selected int32 [slots,
  * kv_heads, top_pages] gets the pages' places in the slot, ascending, then -1. A slot of
- * length 0 gives zeros. Hq / kv_heads <= 16. */
+ * length 0 gives zeros. Hq / kv_heads <= 16, top_pages <= 4096. */
 size_t iron_page_select_attn_workspace_bytes(int batch, int num_heads, int kv_heads, int head_dim, int max_pages,
                                              int top_pages, int page_size);
 int iron_page_select_attn(const iron_page_pool *pool, const uint16_t *q, uint16_t *out, int32_t *selected,

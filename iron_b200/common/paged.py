@@ -44,13 +44,13 @@ class PagedOperator(MLIROperator):
 
     def _workspace(self, stream: int):
         """(address, bytes) of this stream's workspace."""
-        import torch
-
         ws = self._spaces.get(stream)
         if ws is None:
-            ws = torch.empty(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
-            self._spaces[stream] = ws
-        return ws.data_ptr(), ws.numel()
+            import torch
+
+            t = torch.empty(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
+            ws = self._spaces[stream] = (t.data_ptr(), t.numel(), t)
+        return ws[0], ws[1]
 
     def prepare(self):
         self._workspace(_lib.current_stream())
@@ -63,22 +63,28 @@ class PagedOperator(MLIROperator):
 
         if self._wanted is None:
             kinds = {np.dtype(np.int32): torch.int32, np.dtype(np.int8): torch.int8, np.dtype(np.float32): torch.float32}
-            self._wanted = [(int(np.prod(s.shape, dtype=np.int64)), kinds.get(np.dtype(np_dtype(s.dtype)), torch.bfloat16),
-                             tuple(s.shape), i in self._strided) for i, s in enumerate(self.get_arg_spec())]
+            self._wanted = [(kinds.get(np.dtype(np_dtype(s.dtype)), torch.bfloat16), int(np.prod(s.shape, dtype=np.int64)),
+                             s.shape if i in self._strided else None) for i, s in enumerate(self.get_arg_spec())]
         if len(bufs) != len(self._wanted):
             raise ValueError(f"{type(self).__name__} takes {len(self._wanted)} buffers, got {len(bufs)}")
-        for i, (t, (numel, dtype, shape, strided)) in enumerate(zip(bufs, self._wanted)):
-            if not isinstance(t, torch.Tensor):
-                t = t.device_tensor
+        for t, (dtype, numel, view) in zip(bufs, self._wanted):
+            if t.dtype is not dtype or not (t.numel() >= numel if t.is_contiguous() else
+                                            view and t.shape == view and t.stride(-1) == 1):
+                self._refuse_buffers(bufs)
+
+    def _refuse_buffers(self, bufs):
+        """Raises for what is wrong with the buffers."""
+        me = type(self).__name__
+        for i, (t, (dtype, numel, view)) in enumerate(zip(bufs, self._wanted)):
             if t.dtype is not dtype:
-                raise ValueError(f"buffer {i} of {type(self).__name__} is {t.dtype}, needs {dtype}")
+                raise ValueError(f"buffer {i} of {me} is {t.dtype}, needs {dtype}")
             if t.is_contiguous():
                 if t.numel() < numel:
-                    raise ValueError(f"buffer {i} of {type(self).__name__} holds {t.numel()} values, needs {numel}")
-            elif not strided or t.shape != shape:
-                raise ValueError(f"buffer {i} of {type(self).__name__} must be contiguous")
+                    raise ValueError(f"buffer {i} of {me} holds {t.numel()} values, needs {numel}")
+            elif view is None or t.shape != view:
+                raise ValueError(f"buffer {i} of {me} must be contiguous")
             elif t.stride(-1) != 1:
-                raise ValueError(f"buffer {i} of {type(self).__name__} needs a contiguous last dimension")
+                raise ValueError(f"buffer {i} of {me} needs a contiguous last dimension")
 
     def get_callable(self):
         import torch
@@ -89,28 +95,25 @@ class PagedOperator(MLIROperator):
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
         def call(*bufs):
-            check(bufs)
-            launch(*bufs, stream=raw(device()))
+            tensors = [getattr(b, "device_tensor", b) for b in bufs]
+            check(tensors)
+            launch(*tensors, stream=raw(device()))
             for i in written:
-                if not isinstance(bufs[i], torch.Tensor):
+                if bufs[i] is not tensors[i]:
                     bufs[i].mark_device_written()
 
         return call
 
 
 def address(t):
-    """Device address of a CUDA tensor (or of an iron_b200 Tensor)."""
-    try:
-        if t.is_cuda:
-            return t.data_ptr()
-    except AttributeError:
-        pass
-    return _lib.dptr(t)
+    """Device address of a CUDA tensor."""
+    if not t.is_cuda:
+        raise RuntimeError("iron_b200 kernels take CUDA tensors; got a host tensor")
+    return t.data_ptr()
 
 
 def strides(t, shape):
     """Element strides of the leading dimensions of `t` seen as `shape`."""
-    t = getattr(t, "device_tensor", t)
     if t.shape == shape:
         return t.stride()[:-1]
     out, step = [], 1

@@ -581,6 +581,7 @@ extern "C" size_t iron_page_append_workspace_bytes(int slots, int num_pages) {
 extern "C" int iron_page_append(const iron_page_pool *c, const uint16_t *k_new, const uint16_t *v_new,
                                 const int32_t *index, int num_new, int32_t *lens_out, int32_t *status,
                                 void *workspace, size_t workspace_bytes, unsigned flags, void *stream) {
+  (void)flags;
   const int chk = pool_check(c);
   if (chk != IRON_OK) return chk;
   if (!k_new || !v_new || !index || !c->lens || !lens_out || !status || !workspace) return IRON_ERR_NULL;
@@ -612,7 +613,7 @@ extern "C" int iron_page_append(const iron_page_pool *c, const uint16_t *k_new, 
   a.M = c->max_pages;
   a.layer_stride = static_cast<int64_t>(a.P) * a.Hkv * a.page * a.D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int st = launch(append_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, (flags & IRON_FLAG_PDL) != 0, a);
+  int st = launch(append_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, a);
   if (st != IRON_OK) return st;
   const int touched = min((num_new + a.page - 2) / a.page + 1, a.M);
   const int vpr = a.Hkv * a.D / 8, width = vpr < kAppendThreads ? vpr : kAppendThreads;
@@ -634,6 +635,7 @@ extern "C" size_t iron_page_fork_workspace_bytes(int slots) {
 extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, int32_t *page_table_out,
                               int32_t *lens_out, int32_t *refs_out, int32_t *status, void *workspace,
                               size_t workspace_bytes, unsigned flags, void *stream) {
+  (void)flags;
   const int chk = pool_check(c);
   if (chk != IRON_OK) return chk;
   if (!source || !c->lens || !page_table_out || !lens_out || !refs_out || !status || !workspace) return IRON_ERR_NULL;
@@ -668,7 +670,7 @@ extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, in
   a.layer_stride = static_cast<int64_t>(a.P) * a.Hkv * a.page * a.D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int copiers = min(64, (a.P + kPlanThreads - 1) / kPlanThreads);
-  int st = launch(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), 0, s, (flags & IRON_FLAG_PDL) != 0, a);
+  int st = launch(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), 0, s, true, a);
   if (st != IRON_OK) return st;
   return launch(fork_copy_kernel, dim3(sm_count() * 8), dim3(kCopyThreads), 0, s, true, a);
 }
@@ -679,6 +681,7 @@ extern "C" size_t iron_page_compact_workspace_bytes(int num_pages) {
 
 extern "C" int iron_page_compact(const iron_page_pool *c, int32_t *page_table_out, int32_t *refs_out, int32_t *used,
                                  void *workspace, size_t workspace_bytes, unsigned flags, void *stream) {
+  (void)flags;
   const int chk = pool_check(c);
   if (chk != IRON_OK) return chk;
   if (!page_table_out || !refs_out || !used || !workspace) return IRON_ERR_NULL;
@@ -710,7 +713,7 @@ extern "C" int iron_page_compact(const iron_page_pool *c, int32_t *page_table_ou
   a.M = c->max_pages;
   a.layer_stride = static_cast<int64_t>(a.P) * a.Hkv * a.page * a.D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int st = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, (flags & IRON_FLAG_PDL) != 0, a);
+  int st = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, a);
   if (st != IRON_OK) return st;
   return launch(compact_copy_kernel, dim3(sm_count() * 8), dim3(kCopyThreads), 0, s, true, a);
 }

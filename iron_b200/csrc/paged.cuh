@@ -24,36 +24,59 @@ inline int pool_geometry_check(const iron_page_pool *c) {
 }
 
 // ---- a warp's attention over blocks of 16 tokens ------------------------------------------
-// Rows are up to 16 query rows (gid = lane / 4 and gid + 8); tokens come 16 at a time.
-// S = Q K^T takes K fragments straight from the cache rows: the order of k inside an MMA
-// is free as long as Q and K agree, so each lane feeds the 16 contiguous bytes it loaded
-// (k-step ks covers d = 32 (ks / 2) + 8 tid + 4 (ks % 2) + {0, 1 | 2, 3}). V goes through a
-// padded shared tile and ldmatrix.trans.
+// Rows are up to 16 query rows (gid = lane / 4 and gid + 8); tokens come 16 at a time
+// through a ring of shared-memory stages of the warp's own, filled by asynchronous copies
+// kStages - 1 blocks ahead (one block in registers, the form before, kept 4 KB per warp in
+// flight: 2.8 TB/s on B200 at 64 sequences). Rows are padded to an odd number of 16-byte
+// pieces, so that ldmatrix meets no bank conflicts. S = Q K^T and O += P V are mma.sync
+// m16n8k16, the softmax runs online in fp32.
 
+// Asynchronous 16-byte global -> shared copy; zeros instead where !full (nothing is read).
+__device__ __forceinline__ void cp_async16_zfill(void *dst, const void *src, bool full) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(full ? 16 : 0)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], const void *p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p)))
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], const void *p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p)))
+               : "memory");
+}
+
+// A stage: 16 rows of K, then 16 rows of V.
 template <int D>
-struct WarpBlock {
-  uint4 k[2][D / 32];  // K rows gid and gid + 8, 16-byte pieces tid, tid + 4, ...
-  uint4 v[D / 16];     // V pieces i * 32 + lane of the 16 x D tile
+struct Stage {
+  static constexpr int kRow = D + 8;            // elements
+  static constexpr int kElems = 2 * 16 * kRow;  // K and V
+  static constexpr int kBytes = kElems * 2;
+  uint16_t x[kElems];
 
-  // rows >= n are zero and are not read
-  __device__ __forceinline__ void load(const uint16_t *kp, const uint16_t *vp, int64_t krow, int64_t vrow, int n) {
-    const int lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-        k[nt][db] = nt * 8 + gid < n ? ld_act_v4(kp + (nt * 8 + gid) * krow + db * 32 + tid * 8) : make_uint4(0, 0, 0, 0);
+  // rows >= n become zero and are not read (n <= 0: none is)
+  __device__ __forceinline__ void load(const uint16_t *k, const uint16_t *v, int64_t krow, int64_t vrow, int n) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const int idx = i * 32 + lane, row = idx / (D / 8), c = idx % (D / 8);
-      v[i] = row < n ? ld_act_v4(vp + row * vrow + c * 8) : make_uint4(0, 0, 0, 0);
+      cp_async16_zfill(x + row * kRow + c * 8, row < n ? k + row * krow + c * 8 : k, row < n);
+      cp_async16_zfill(x + (16 + row) * kRow + c * 8, row < n ? v + row * vrow + c * 8 : v, row < n);
     }
   }
 };
 
 template <int D>
 struct WarpAttn {
-  static constexpr int kVStride = D + 8;  // padded V row: an odd number of 16-byte pieces
   uint32_t q[D / 16][4];
   float o[D / 8][4];
   float m[2], l[2];  // running maximum (log2 units) and this lane's share of the sum, rows gid and gid + 8
@@ -70,37 +93,27 @@ struct WarpAttn {
     const int tid = threadIdx.x & 3;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      const int d = 32 * (ks >> 1) + 8 * tid + 4 * (ks & 1);
-      const uint2 a = lo ? ld_act_v2(lo + d) : make_uint2(0, 0), b = hi ? ld_act_v2(hi + d) : make_uint2(0, 0);
-      q[ks][0] = a.x;
-      q[ks][1] = b.x;
-      q[ks][2] = a.y;
-      q[ks][3] = b.y;
+      const int d = 16 * ks + 2 * tid;
+      q[ks][0] = lo ? ld_act_u32(lo + d) : 0u;
+      q[ks][1] = hi ? ld_act_u32(hi + d) : 0u;
+      q[ks][2] = lo ? ld_act_u32(lo + d + 8) : 0u;
+      q[ks][3] = hi ? ld_act_u32(hi + d + 8) : 0u;
     }
   }
 
-  __device__ __forceinline__ void stage_v(const WarpBlock<D> &x, uint16_t *vs) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const int idx = i * 32 + lane, row = idx / (D / 8), c = idx % (D / 8);
-      *reinterpret_cast<uint4 *>(vs + row * kVStride + c * 8) = x.v[i];
-    }
-  }
-
-  // One block whose V tile is staged in vs (stage_v, same warp); bit t of see[0] / see[1]:
-  // row gid / gid + 8 sees token t.
-  __device__ __forceinline__ void step(const uint4 (&k)[2][D / 32], const uint16_t *vs, float scale_log2,
-                                       const uint32_t (&see)[2]) {
+  // One block; bit t of see[0] / see[1]: row gid / gid + 8 sees token t.
+  __device__ __forceinline__ void step(const Stage<D> &st, float scale_log2, const uint32_t (&see)[2]) {
     const int lane = threadIdx.x & 31, tid = lane & 3;
     float s[2][4];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
       s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint4 &w = k[nt][ks >> 1];
-        mma_bf16_16816(s[nt], q[ks], (ks & 1) ? w.z : w.x, (ks & 1) ? w.w : w.y);
+      for (int j = 0; j < D / 32; ++j) {
+        uint32_t b[4];
+        ldsm_x4(b, st.x + (nt * 8 + (lane & 7)) * Stage<D>::kRow + (4 * j + (lane >> 3)) * 8);
+        mma_bf16_16816(s[nt], q[2 * j], b[0], b[1]);
+        mma_bf16_16816(s[nt], q[2 * j + 1], b[2], b[3]);
       }
     }
     float mx[2] = {-INFINITY, -INFINITY};
@@ -149,22 +162,15 @@ struct WarpAttn {
       hi[i] = pack_bf16x2(p0, p1);
       lo[i] = pack_bf16x2(p0 - bf16_lo(hi[i]), p1 - bf16_hi(hi[i]));
     }
-    __syncwarp();  // V tile stores visible to ldmatrix
 #pragma unroll
     for (int jp = 0; jp < D / 16; ++jp) {
-      const int row = (lane & 7) + ((lane >> 3) & 1) * 8, col = jp * 16 + (lane >> 4) * 8;
-      const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(vs + row * kVStride + col));
       uint32_t b[4];
-      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
-                   : "r"(addr)
-                   : "memory");
+      ldsm_x4_t(b, st.x + (16 + (lane & 7) + ((lane >> 3) & 1) * 8) * Stage<D>::kRow + jp * 16 + (lane >> 4) * 8);
       mma_bf16_16816(o[2 * jp], hi, b[0], b[1]);
       mma_bf16_16816(o[2 * jp + 1], hi, b[2], b[3]);
       mma_bf16_16816(o[2 * jp], lo, b[0], b[1]);
       mma_bf16_16816(o[2 * jp + 1], lo, b[2], b[3]);
     }
-    __syncwarp();  // done with the V tile before it is staged again
   }
 
   // the row sums over the four lanes of each row

@@ -194,6 +194,6 @@ static_assert(kTMaxNodes == 128, "four words of 32 nodes");
 
 // The tcgen05 form (tree_attention_tc.cu).
 size_t tree_tc_workspace(int head_dim);
-int tree_tc_launch(TreeArgs a, int head_dim, bool pdl, cudaStream_t s);
+int tree_tc_launch(TreeArgs a, int head_dim, cudaStream_t s);
 
 }  // namespace iron

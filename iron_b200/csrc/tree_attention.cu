@@ -15,24 +15,30 @@ namespace iron {
 constexpr int kTRows = 16;     // rows per unit
 constexpr int kTTile = 64;     // tokens per tile: 16 per warp
 constexpr int kTWarps = 4;
-constexpr int kTCtasPerSm = 4;
 struct TreeCut {
   static constexpr int kTile = kTTile, kUnitCost = 1;
 };
 
 template <int D>
-__global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(TreeArgs a) {
-  using Attn = WarpAttn<D>;
-  constexpr int kVBytes = kTWarps * 16 * Attn::kVStride * 2;
-  constexpr int kOBytes = kTWarps * kTRows * D * 4;
-  __shared__ __align__(16) uint8_t smem[kVBytes > kOBytes ? kVBytes : kOBytes];  // V tiles, then the merge
+struct TreeCfg {
+  static constexpr int kStages = 3, kCtasPerSm = D == 64 ? 3 : 2;
+  static constexpr int kRing = kTWarps * kStages * Stage<D>::kBytes;  // the stages; after them the merge
+  static constexpr int kMerge = kTWarps * kTRows * D * 4;
+  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+};
+
+template <int D>
+__global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_attn_kernel(TreeArgs a) {
+  using C = TreeCfg<D>;
+  constexpr int kStages = C::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red_m[kTWarps][kTRows], red_l[kTWarps][kTRows];
   __shared__ int pref[kTMaxBatch + 1], warp_sums[kTWarps];
   __shared__ TreePaths tree;
   __shared__ __align__(16) uint32_t paths[kTRows][kTMaxNodes / 32];
   __shared__ uint32_t usable[kTMaxNodes / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
-  uint16_t *vs = reinterpret_cast<uint16_t *>(smem) + warp * 16 * Attn::kVStride;
+  Stage<D> *ring = reinterpret_cast<Stage<D> *>(smem) + warp * kStages;
   float (*red_o)[kTRows][D] = reinterpret_cast<float (*)[kTRows][D]>(smem);
   pdl_launch_dependents();
   pdl_wait();
@@ -50,8 +56,32 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
     const int b = sg.b, h = sg.h, row0 = sg.group * kTRows, first = sg.first, count = sg.count;
     const int len = cached_len(a, b), ctiles = (len + kTTile - 1) / kTTile;
     const int *table = a.table + static_cast<int64_t>(b) * a.M;
+    // the warp's blocks: cached tiles first .. ctiles - 1 (block 4 i + warp of tokens), then nodes
+    const int ncached = max(0, min(first + count, ctiles) - first);
+    // page of the cached block of tile first + i: 32 of them per load, one per lane
+    auto entry = [&](int i) {
+      const int t = (first + i + lane) * kTTile + warp * 16;
+      return i + lane < ncached && t < len ? ld_act_i32(table + (t >> a.page_shift)) : -1;
+    };
+    int pages = entry(0);
+    auto request = [&](int i, int stage) {  // block of tile first + i
+      if (i < ncached) {
+        if ((i & 31) == 0 && i > 0) pages = entry(i);
+        const int p = __shfl_sync(0xffffffffu, pages, i & 31), t = (first + i) * kTTile + warp * 16;
+        const int n = p >= 0 && p < a.P ? min(16, len - t) : 0;
+        const int64_t at0 = n > 0 ? (((static_cast<int64_t>(p) * a.Hkv + h) << a.page_shift) + (t & (page - 1))) * D : 0;
+        ring[stage].load(a.k + at0, a.v + at0, D, D, n);
+        cp_async_commit();
+        return n;
+      }
+      cp_async_commit();
+      return 0;
+    };
+    int valid[kStages];  // tokens of the blocks in flight
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) valid[s] = request(s, s);
 
-    Attn at;
+    WarpAttn<D> at;
     at.clear();
     const int r_lo = row0 + gid, r_hi = row0 + gid + 8, rows = a.N * g;
     const uint16_t *qb = a.q + b * a.qs[0];
@@ -72,56 +102,70 @@ __global__ void __launch_bounds__(32 * kTWarps, kTCtasPerSm) tree_attn_kernel(Tr
       }
       __syncthreads();
     }
-    WarpBlock<D> blk;
-    for (int i = first; i < first + count; ++i) {
-      uint32_t see[2];
-      if (i < ctiles) {
-        const int t = i * kTTile + warp * 16, n = min(16, len - t);
-        if (n <= 0) continue;
-        const int p = ld_act_i32(table + (t >> a.page_shift));
-        const bool ok = p >= 0 && p < a.P;
-        const int64_t at0 = ((static_cast<int64_t>(ok ? p : 0) * a.Hkv + h) << a.page_shift) + (t & (page - 1));
-        blk.load(a.k + at0 * D, a.v + at0 * D, D, D, ok ? n : 0);
-        see[0] = see[1] = ok ? 0xffffu >> (16 - n) : 0u;
-      } else {
-        const int j0 = (i - ctiles) * kTTile + warp * 16;
-        if (j0 >= a.N) continue;
-        const uint32_t can = usable[j0 >> 5] >> (j0 & 31) & 0xffffu;
-        const int64_t at0 = b * a.ks[0] + j0 * a.ks[1] + h * a.ks[2];
-        // unused nodes are not read: rows past the last usable one by n, others by the mask
-        blk.load(a.k_new + at0, a.v_new + at0, a.ks[1], a.ks[1], can ? 32 - __clz(can) : 0);
-        see[0] = paths[gid][j0 >> 5] >> (j0 & 31) & 0xffffu;
-        see[1] = paths[gid + 8][j0 >> 5] >> (j0 & 31) & 0xffffu;
-        // a masked token's probability is 0, but 0 * inf is not: values that are not finite
-        // leave the tile and are added to the rows that see them
-        bool odd = false;
+    for (int i0 = 0; i0 < ncached; i0 += kStages) {
 #pragma unroll
-        for (int v = 0; v < D / 16; ++v) {
-          uint32_t *e = reinterpret_cast<uint32_t *>(&blk.v[v]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if ((e[c] & 0x7f80u) == 0x7f80u) e[c] &= 0xffff0000u, odd = true;
-            if ((e[c] & 0x7f800000u) == 0x7f800000u) e[c] &= 0xffffu, odd = true;
-          }
-        }
-        if (__any_sync(0xffffffffu, odd)) {
-          for (int t = 0; t < 16; ++t) {
-            if (!(can >> t & 1u)) continue;
-            const uint16_t *vt = a.v_new + at0 + t * a.ks[1];
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float f = bf16_bits_to_float(ld_act_u16(vt + 8 * j + 2 * tid + e));
-                if (isfinite(f)) continue;
-                if (see[0] >> t & 1u) at.o[j][e] += f;
-                if (see[1] >> t & 1u) at.o[j][2 + e] += f;
-              }
-          }
+      for (int s = 0; s < kStages; ++s) {
+        const int i = i0 + s;
+        if (i >= ncached) break;
+        cp_async_wait<kStages - 2>();
+        __syncwarp();  // the block is here, and every lane is done with the stage refilled next
+        constexpr int kLast = kStages - 1;
+        valid[(s + kLast) % kStages] = request(i + kLast, (s + kLast) % kStages);
+        if (valid[s] > 0) {
+          const uint32_t see[2] = {0xffffu >> (16 - valid[s]), 0xffffu >> (16 - valid[s])};
+          at.step(ring[s], a.scale_log2, see);
         }
       }
-      at.stage_v(blk, vs);
-      at.step(blk.k, vs, a.scale_log2, see);
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    for (int i = max(first, ctiles); i < first + count; ++i) {
+      const int j0 = (i - ctiles) * kTTile + warp * 16;
+      if (j0 >= a.N) continue;
+      const uint32_t can = usable[j0 >> 5] >> (j0 & 31) & 0xffffu;
+      const int64_t at0 = b * a.ks[0] + j0 * a.ks[1] + h * a.ks[2];
+      Stage<D> &st = ring[0];
+      st.load(a.k_new + at0, a.v_new + at0, a.ks[1], a.ks[1], can ? 32 - __clz(can) : 0);
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
+      const uint32_t see[2] = {paths[gid][j0 >> 5] >> (j0 & 31) & 0xffffu, paths[gid + 8][j0 >> 5] >> (j0 & 31) & 0xffffu};
+      // a masked token's probability is 0, but 0 * inf is not: values that are not finite
+      // leave the tile and are added to the rows that see them
+      bool odd = false;
+#pragma unroll
+      for (int v = 0; v < D / 16; ++v) {
+        const int idx = v * 32 + lane;
+        uint4 *p = reinterpret_cast<uint4 *>(st.x + (16 + idx / (D / 8)) * Stage<D>::kRow + idx % (D / 8) * 8);
+        uint4 y = *p;
+        uint32_t *e = reinterpret_cast<uint32_t *>(&y);
+        bool change = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if ((e[c] & 0x7f80u) == 0x7f80u) e[c] &= 0xffff0000u, change = true;
+          if ((e[c] & 0x7f800000u) == 0x7f800000u) e[c] &= 0xffffu, change = true;
+        }
+        if (change) *p = y;
+        odd |= change;
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+        __syncwarp();
+        for (int t = 0; t < 16; ++t) {
+          if (!(can >> t & 1u)) continue;
+          const uint16_t *vt = a.v_new + at0 + t * a.ks[1];
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float f = bf16_bits_to_float(ld_act_u16(vt + 8 * j + 2 * tid + e));
+              if (isfinite(f)) continue;
+              if (see[0] >> t & 1u) at.o[j][e] += f;
+              if (see[1] >> t & 1u) at.o[j][2 + e] += f;
+            }
+        }
+      }
+      at.step(st, a.scale_log2, see);
+      __syncwarp();  // done with the stage
     }
     at.finish();
     __syncthreads();  // every warp is done with the V tiles
@@ -229,11 +273,13 @@ __global__ void __launch_bounds__(kTRows *D / 4) tree_join_kernel(TreeArgs a, in
 
 using namespace iron;
 
-static int tree_pieces() { return sm_count() * kTCtasPerSm; }
+static int tree_pieces(int head_dim) {
+  return sm_count() * (head_dim == 128 ? TreeCfg<128>::kCtasPerSm : TreeCfg<64>::kCtasPerSm);
+}
 
 extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
   if (batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  const size_t few = static_cast<size_t>(tree_pieces()) * 2 * kTRows * (2 + head_dim) * sizeof(float);
+  const size_t few = static_cast<size_t>(tree_pieces(head_dim)) * 2 * kTRows * (2 + head_dim) * sizeof(float);
   const size_t many = tree_tc_workspace(head_dim);
   return few > many ? few : many;
 }
@@ -255,6 +301,7 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
                               const int32_t *parents, uint16_t *out, int num_nodes, int num_heads,
                               const int64_t *q_strides, const int64_t *kv_strides, const int64_t *out_strides,
                               float scale, void *workspace, size_t workspace_bytes, unsigned flags, void *stream) {
+  (void)flags;
   const int chk = pool_geometry_check(c);
   if (chk != IRON_OK) return chk;
   if (!c->lens || !q || !k_new || !v_new || !parents || !out || !q_strides || !kv_strides || !out_strides || !workspace)
@@ -294,10 +341,19 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.P = c->num_pages;
   a.scale_log2 = scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool pdl = (flags & IRON_FLAG_PDL) != 0, wide = c->head_dim == 128;
-  if (use_tensor_form(a)) return tree_tc_launch(a, c->head_dim, pdl, s);
-  const int pieces = tree_pieces();
-  int st = launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps), 0, s, pdl, a);
+  const bool wide = c->head_dim == 128;
+  if (use_tensor_form(a)) return tree_tc_launch(a, c->head_dim, s);
+  const int pieces = tree_pieces(c->head_dim);
+  static PerDeviceOnce once;
+  int st = once.run([] {
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeCfg<64>::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(tree_attn_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeCfg<128>::kSmem);
+    return call_status(e);
+  });
+  if (st != IRON_OK) return st;
+  st = launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps),
+              wide ? TreeCfg<128>::kSmem : TreeCfg<64>::kSmem, s, true, a);
   if (st != IRON_OK) return st;
   return launch(wide ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv * a.groups),
                 dim3(wide ? kTRows * 32 : kTRows * 16), 0, s, true, a, pieces);

@@ -734,7 +734,7 @@ static int make_map(CUtensorMap *m, const void *ptr, const uint64_t (&dims)[4], 
 }
 
 template <int D>
-static int launch_tc(TreeArgs a, bool pdl, cudaStream_t s) {
+static int launch_tc(TreeArgs a, cudaStream_t s) {
   using C = Cfg<D>;
   static PerDeviceOnce once;
   const int st0 = once.run([] {
@@ -754,7 +754,7 @@ static int launch_tc(TreeArgs a, bool pdl, cudaStream_t s) {
   if (st == IRON_OK) st = make_map(&maps.v_new, a.v_new, nd, ns, kTile);
   if (st != IRON_OK) return st;
   const int ctas = sm_count();
-  st = launch(tree_tc_kernel<D>, dim3(ctas), dim3(kThreads), C::kSmem, s, pdl, maps, a);
+  st = launch(tree_tc_kernel<D>, dim3(ctas), dim3(kThreads), C::kSmem, s, true, maps, a);
   if (st != IRON_OK) return st;
   const int rows = a.N * (a.Hq / a.Hkv);
   return launch(tree_tc_join_kernel<D>, dim3(a.B * a.Hkv * a.groups, ((rows < 256 ? rows : 256) + 31) / 32), dim3(256), 0, s,
@@ -768,8 +768,8 @@ size_t tree_tc_workspace(int head_dim) {
   return static_cast<size_t>(sm_count()) * 4 * part * sizeof(float);
 }
 
-int tree_tc_launch(TreeArgs a, int head_dim, bool pdl, cudaStream_t s) {
-  return head_dim == 128 ? treetc::launch_tc<128>(a, pdl, s) : treetc::launch_tc<64>(a, pdl, s);
+int tree_tc_launch(TreeArgs a, int head_dim, cudaStream_t s) {
+  return head_dim == 128 ? treetc::launch_tc<128>(a, s) : treetc::launch_tc<64>(a, s);
 }
 
 }  // namespace iron

@@ -51,8 +51,8 @@ class PageSelectAttention(PagedOperator):
     def __post_init__(self):
         if not 1 <= self.batch <= 65535:
             raise ValueError(f"batch must be 1 to 65535, got {self.batch}")
-        if self.top_pages < 1:
-            raise ValueError(f"top_pages must be positive, got {self.top_pages}")
+        if not 1 <= self.top_pages <= 4096:
+            raise ValueError(f"top_pages must be 1 to 4096, got {self.top_pages}")
         if self.num_kv_heads < 1 or self.num_heads % self.num_kv_heads or not 1 <= self.num_heads // self.num_kv_heads <= 16:
             raise ValueError("num_heads must be a multiple of num_kv_heads (group <= 16)")
         self._check_geometry()
