@@ -73,6 +73,10 @@ struct Cfg {
   // tables of paths in flight: preparing tile i means that tile i - kStages is done with
   static constexpr int kTrees = kStages + 3;
   static constexpr int kPanels = D / 64;
+  static constexpr int kScores = D == 64 ? 128 : 64;       // tokens of one S
+  // TMEM columns: S of both streams, O of both, P (64 tokens, hi then lo) of both
+  static constexpr int kTmemS = 0, kTmemO = 2 * kScores, kTmemP = kTmemO + 2 * D;
+  static_assert(kTmemP + 128 == 512, "TMEM is full");
   static constexpr uint32_t kPanel = kTile * 128;          // 128 rows x 64 bf16
   static constexpr uint32_t kOperand = kPanels * kPanel;   // Q tile, K tile or V tile
   static constexpr uint32_t kSmem = 1024 + 2 * kOperand + 2 * kStages * kOperand;
@@ -104,20 +108,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// A value that is the same in all lanes, in a form the compiler knows to be so: loops and
+// addresses derived from it stay in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 struct Bars {  // mbarrier addresses
   uint32_t base;
   template <int S> __device__ uint32_t kfull(int i) const { return base + 8 * i; }
   template <int S> __device__ uint32_t kempty(int i) const { return base + 8 * (S + i); }
   template <int S> __device__ uint32_t vfull(int i) const { return base + 8 * (2 * S + i); }
   template <int S> __device__ uint32_t vempty(int i) const { return base + 8 * (3 * S + i); }
-  template <int S> __device__ uint32_t sfull(int i) const { return base + 8 * (4 * S + i); }
-  template <int S> __device__ uint32_t pfull(int i) const { return base + 8 * (4 * S + 2 + i); }
-  template <int S> __device__ uint32_t plast(int i) const { return base + 8 * (4 * S + 4 + i); }
-  template <int S> __device__ uint32_t ofull(int i) const { return base + 8 * (4 * S + 6 + i); }
+  template <int S> __device__ uint32_t sfull(int s) const { return base + 8 * (4 * S + s); }
+  template <int S> __device__ uint32_t sfree(int s) const { return base + 8 * (4 * S + 2 + s); }
+  template <int S> __device__ uint32_t pfull(int s) const { return base + 8 * (4 * S + 4 + s); }
+  template <int S> __device__ uint32_t pvdone(int s) const { return base + 8 * (4 * S + 6 + s); }
   template <int S> __device__ uint32_t qfull(int i) const { return base + 8 * (4 * S + 8 + i); }
   template <int S> __device__ uint32_t vready(int i) const { return base + 8 * (4 * S + 14 + kMasks + i); }
   template <int S> __device__ uint32_t paths(int i) const { return base + 8 * (5 * S + 14 + kMasks + i); }
-  template <int S> __device__ uint32_t drain() const { return base + 8 * (4 * S + 11); }
+  template <int S> __device__ uint32_t drain(int s) const { return base + 8 * (4 * S + 10 + s); }
   template <int S> __device__ uint32_t other() const { return base + 8 * (4 * S + 12); }
   template <int S> __device__ uint32_t joined() const { return base + 8 * (4 * S + 13); }
   template <int S> __device__ uint32_t mask(int i) const { return base + 8 * (4 * S + 14 + i); }
@@ -139,6 +147,11 @@ __device__ __forceinline__ Streams streams_of(const TreeArgs &a, const Segment &
   st.n[0] = st.both ? sg.count : (sg.count + 1) / 2;
   st.n[1] = st.both ? sg.count : sg.count / 2;
   return st;
+}
+
+// Halves of a tile that hold something: a short last tile has one.
+__device__ __forceinline__ int halves_of(const TreeArgs &a, int i, int ctiles, int len) {
+  return (i >= ctiles ? a.N - (i - ctiles) * kTile : len - i * kTile) > kTile / 2 ? 2 : 1;
 }
 
 template <int D>
@@ -169,17 +182,22 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
   const int64_t w_begin = piece_start(total, blockIdx.x, pieces), w_end = piece_start(total, blockIdx.x + 1, pieces);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4 * S; ++i) tc::mbar_init_u32(bars.base + 8 * i, 1);
+    for (int i = 0; i < S; ++i) {
+      tc::mbar_init_u32(bars.kfull<S>(i), 1);
+      tc::mbar_init_u32(bars.kempty<S>(i), 2);
+      tc::mbar_init_u32(bars.vfull<S>(i), 1);
+      tc::mbar_init_u32(bars.vempty<S>(i), 2);
+    }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init_u32(bars.sfull<S>(i), 1);
+      tc::mbar_init_u32(bars.sfree<S>(i), 4);
       tc::mbar_init_u32(bars.pfull<S>(i), 4);
-      tc::mbar_init_u32(bars.plast<S>(i), 4);
-      tc::mbar_init_u32(bars.ofull<S>(i), 1);
+      tc::mbar_init_u32(bars.pvdone<S>(i), 1);
       tc::mbar_init_u32(bars.qfull<S>(i), 4);
     }
-    for (int i = 0; i < S; ++i) tc::mbar_init_u32(bars.vready<S>(i), 2);
+    for (int i = 0; i < S; ++i) tc::mbar_init_u32(bars.vready<S>(i), 1);
     for (int i = 0; i < C::kTrees; ++i) tc::mbar_init_u32(bars.paths<S>(i), 1);
-    tc::mbar_init_u32(bars.drain<S>(), 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init_u32(bars.drain<S>(i), 1);
     for (int i = 0; i < kMasks; ++i) tc::mbar_init_u32(bars.mask<S>(i), 1);
     tc::mbar_init_u32(bars.other<S>(), 4);
     tc::mbar_init_u32(bars.joined<S>(), 4);
@@ -195,7 +213,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 9) {
+    if (warp == 10) {
     // ---- loads ----
     if (lane == 0) {
       tc::prefetch_tmap(&maps.k);
@@ -275,89 +293,101 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         wait_phase(bars.vfull<S>(j % S), (j / S) & 1);
       }
     }
-    } else if (warp == 8) {
-    // ---- MMAs: the warp stays converged, an elected lane issues ----
-    constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, kTile);
+    } else if (warp < 10) {
+    // ---- MMAs of stream `s`: the warp stays converged, an elected lane issues. (One warp for
+    // both streams was what bound the kernel: its instructions share their scheduler with
+    // two softmax warps, and each stream waited for the other one's turn.) ----
+    const int s = warp - 8;
+    constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, C::kScores);
     constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
     bool ok = true;
     int it0 = 0;
-    uint32_t pc[2] = {0, 0}, qc[2] = {0, 0};
-    auto ready = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_phase(bar, parity)) != 0; };
-    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+    uint32_t pc = 0, qc = 0, sn = 0;
+    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); uniform(sg.count) > 0;
          sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
       const Streams st = streams_of(a, sg);
-      auto tile_of = [&](int s, int j) { return it0 + (st.both ? j : 2 * j + s); };
-      auto scores = [&](int s, int j) {
-        const int it = tile_of(s, j), slot = it % S;
-        ok = ready(bars.kfull<S>(slot), (it / S) & 1);
-        if (!ok) return;
+      const int len = uniform(cached_len(a, sg.b)), ctiles = (len + kTile - 1) / kTile;
+      const int first = uniform(sg.first), n = uniform(st.n[s]);
+      const bool both = uniform(st.both);
+      const int it0s = it0 + (both ? 0 : s), step = both ? 1 : 2;
+      // K and V are released by both streams; a tile that one stream has alone, by it twice
+      const bool twice = !both;
+      auto halves = [&](int j) { return halves_of(a, first + (both ? j : 2 * j + s), ctiles, len); };
+      // S of tile j: all of it (h = 0), or its half h
+      auto scores = [&](int j, int h, bool last) {
+        const int it = it0s + j * step, slot = it % S;
+        ok &= wait_phase(bars.kfull<S>(slot), (it / S) & 1);
+        if (sn > 0) ok &= wait_phase(bars.sfree<S>(s), (sn - 1) & 1);
+        ++sn;
         tc::fence_after_sync();
         // a step of the start address is a step of the descriptor's low bits (16-byte units)
         const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
-        const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand);
+        const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand + h * (C::kPanel / 2));
         if (tc::elect_one()) {
 #pragma unroll
           for (int c = 0; c < C::kPanels; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              tc::mma_bf16(tmem + s * 128, q + c * (C::kPanel >> 4) + kk * 2, k + c * (C::kPanel >> 4) + kk * 2, idesc_s,
-                           c > 0 || kk > 0);
+              tc::mma_bf16(tmem + C::kTmemS + s * C::kScores, q + c * (C::kPanel >> 4) + kk * 2,
+                           k + c * (C::kPanel >> 4) + kk * 2, idesc_s, c > 0 || kk > 0);
           tc::mma_commit(bars.sfull<S>(s));
-          if (!st.both || s == 1) tc::mma_commit(bars.kempty<S>(slot));
+          if (last) {
+            tc::mma_commit(bars.kempty<S>(slot));
+            if (twice) tc::mma_commit(bars.kempty<S>(slot));
+          }
         }
         __syncwarp();
       };
-      // in two halves of 64 tokens: the first runs while the second's softmax does
-      auto values = [&](int s, int j) {
-        const int it = tile_of(s, j), slot = it % S;
-        const uint32_t p = tmem + s * 128, o = tmem + 256 + s * D, parity = pc[s]++ & 1;
-        const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand, C::kPanel);
-        ok = ready(bars.vready<S>(slot), (it / S) & 1) && ready(bars.pfull<S>(s), parity);
-        if (!ok) return;
+      auto values = [&](int j, int h, bool last) {
+        const int it = it0s + j * step, slot = it % S;
+        ok &= wait_phase(bars.vready<S>(slot), (it / S) & 1);
+        ok &= wait_phase(bars.pfull<S>(s), pc++ & 1);
         tc::fence_after_sync();
+        const uint32_t p = tmem + C::kTmemP + s * 64, o = tmem + C::kTmemO + s * D;
+        const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand + h * (C::kPanel / 2), C::kPanel);
         if (tc::elect_one()) {
 #pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              tc::mma_bf16_ts(o, p + part * 64 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || part > 0 || kk > 0);
-        }
-        __syncwarp();
-        ok = ready(bars.plast<S>(s), parity);
-        if (!ok) return;
-        tc::fence_after_sync();
-        if (tc::elect_one()) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int kk = 4; kk < 8; ++kk)
-              tc::mma_bf16_ts(o, p + part * 64 + kk * 8, v + kk * (2048 >> 4), idesc_o, 1);
-          if (!st.both || s == 1) tc::mma_commit(bars.vempty<S>(slot));
-          if (j == st.n[s] - 1) tc::mma_commit(bars.ofull<S>(s));
+              tc::mma_bf16_ts(o, p + part * 32 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || h > 0 || part > 0 || kk > 0);
+          tc::mma_commit(bars.pvdone<S>(s));
+          if (last) {
+            tc::mma_commit(bars.vempty<S>(slot));
+            if (twice) tc::mma_commit(bars.vempty<S>(slot));
+          }
         }
         __syncwarp();
       };
-      for (int s = 0; s < 2; ++s)
-        if (st.n[s] > 0 && ok) {
-          ok = ready(bars.qfull<S>(s), qc[s]++ & 1);
-          if (ok) scores(s, 0);
-        }
-      for (int j = 0; j < st.n[0] && ok; ++j)
-        for (int s = 0; s < 2; ++s)
-          if (j < st.n[s]) {
-            if (ok) values(s, j);
-            if (ok && j + 1 < st.n[s]) scores(s, j + 1);
+      if (n > 0) {
+        ok &= wait_phase(bars.qfull<S>(s), qc++ & 1);
+        int k = halves(0);
+        scores(0, 0, C::kScores == kTile || k == 1);
+        // the S that follows goes out before the P V of the last half that the present S
+        // holds: it runs while that half's softmax does, and the softmax never waits for it
+        for (int j = 0; j < n; ++j) {
+          const int next = j + 1 < n ? halves(j + 1) : 0;
+          for (int h = 0; h < k; ++h) {
+            if (C::kScores < kTile && h + 1 < k) scores(j, h + 1, h + 2 == k);
+            else if (h + 1 == k && next > 0) scores(j + 1, 0, C::kScores == kTile || next == 1);
+            values(j, h, h + 1 == k);
           }
-      it0 += sg.count;
+          k = next;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+      }
+      if (!ok) break;
+      it0 += uniform(sg.count);
     }
     if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
     // every MMA issued is done before TMEM is freed
-    if (tc::elect_one()) tc::mma_commit(bars.drain<S>());
+    if (tc::elect_one()) tc::mma_commit(bars.drain<S>(s));
     __syncwarp();
-    wait_phase(bars.drain<S>(), 0);
+    wait_phase(bars.drain<S>(s), 0);
     __syncwarp();
     } else {
-    // ---- preparation: warp 10 and 11 ----
+    // ---- preparation: warp 11 ----
     bool ok = true;
     int it = 0, trees_done = 0;
     for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
@@ -365,13 +395,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       const int ctiles = (cached_len(a, sg.b) + kTile - 1) / kTile;
       TreePaths &tree = trees[trees_done % C::kTrees];
       if (sg.first + sg.count > ctiles) {
-        if (warp == 10) {
-          tree_paths(tree, a.parents + static_cast<int64_t>(sg.b) * a.N, a.N);
-          if (lane == 0) tc::arrive(bars.paths<S>(trees_done % C::kTrees));
-        } else {
-          ok = __all_sync(0xffffffffu, wait_phase(bars.paths<S>(trees_done % C::kTrees), (trees_done / C::kTrees) & 1));
-          if (!ok) break;
-        }
+        tree_paths(tree, a.parents + static_cast<int64_t>(sg.b) * a.N, a.N);
+        tc::arrive_if(lane == 0, bars.paths<S>(trees_done % C::kTrees));
         ++trees_done;
       }
       for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
@@ -385,7 +410,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           // finite (0 * inf is not 0; rows that see them get them added at the end)
           bool odd = false;
 #pragma unroll 1
-          for (int r = (warp - 10) * 32 + lane; r < kTile; r += 64) {
+          for (int r = lane; r < kTile; r += 32) {
             const bool keep = nodes ? tree.up[r] == -1 : masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
             if (keep && !nodes) continue;
             uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
@@ -410,7 +435,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           tc::fence_proxy_async_smem();
         }
         __syncwarp();
-        if (lane == 0) tc::arrive(bars.vready<S>(slot));
+        tc::arrive_if(lane == 0, bars.vready<S>(slot));
       }
     }
     if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 5u);
@@ -420,11 +445,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     // ---- softmax of one stream: thread = row ----
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
+    const uint32_t to = tmem + lanes + C::kTmemO + s * D, tp = tmem + lanes + C::kTmemP + s * 64;
     uint8_t *qs = smem + s * C::kOperand;
     bool ok = true;
     int it0 = 0;
-    uint32_t sc = 0, oc = 0, jc = 0;
+    uint32_t sc = 0 /* S of this stream */, vc = 0 /* P V */, jc = 0;
     int trees_seen = 0;
     // The stream's rows of Q into shared memory, swizzled as TMA would write them (16-byte
     // piece c of row r at c ^ (r % 8)): 8 lanes per row and panel of 64. The first S of the
@@ -451,7 +476,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tc::arrive(bars.qfull<S>(s));
+      tc::arrive_if(lane == 0, bars.qfull<S>(s));
     };
     Segment sg = next_segment<Cut>(a, pref, w_begin, w_end);
     Streams st = streams_of(a, sg);
@@ -465,79 +490,84 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       const int node = live ? row / g : 0, hq = h * g + (live ? row % g : 0);
       float m = -INFINITY, l = 0.f;
       uint4 path = make_uint4(0u, 0u, 0u, 0u);
-      for (int j = 0; j < n; ++j) {
-        const int i = sg.first + (st.both ? j : 2 * j + s), it = it0 + i - sg.first, slot = it % S;
-        // (the masks have barriers of their own: K's may be a phase further by now)
-        ok = __all_sync(0xffffffffu, wait_phase(bars.sfull<S>(s), sc++ & 1) &&
-                                         wait_phase(bars.mask<S>(it % kMasks), (it / kMasks) & 1));
-        if (!ok) break;
-        tc::fence_after_sync();
-        uint32_t x[128];
-        tc::tmem_ld64(ts, x);
-        tc::tmem_ld64(ts + 64, x + 64);
+      bool huge = false;
+      for (int j = 0; j < n && ok; ++j) {
+        const int i = sg.first + (st.both ? j : 2 * j + s), it = it0 + i - sg.first;
         const bool nodes = i >= ctiles;
-        if (has_tree && j == n - 1) {  // the row's path, while its table is there
-          ok = __all_sync(0xffffffffu, wait_phase(bars.paths<S>(trees_seen % C::kTrees), (trees_seen / C::kTrees) & 1));
+        uint4 see;
+#pragma unroll 1
+        for (int half = 0, halves = halves_of(a, i, ctiles, len); half < halves; ++half) {
+          const uint32_t ts = tmem + lanes + C::kTmemS + s * C::kScores + (C::kScores == kTile ? half * 64 : 0);
+          if (half == 0 || C::kScores < kTile) ok = __all_sync(0xffffffffu, wait_phase(bars.sfull<S>(s), sc++ & 1));
+          if (ok && half == 0) {
+            // (the masks have barriers of their own: K's may be a phase further by now)
+            ok = __all_sync(0xffffffffu, wait_phase(bars.mask<S>(it % kMasks), (it / kMasks) & 1));
+            if (ok && has_tree && j == n - 1) {  // the row's path, while its table is there
+              const int t = trees_seen % C::kTrees;
+              ok = __all_sync(0xffffffffu, wait_phase(bars.paths<S>(t), (trees_seen / C::kTrees) & 1));
+              if (ok && live) path = trees[t].bits[node];
+            }
+            see = nodes ? path : *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
+          }
           if (!ok) break;
-          if (live) path = trees[trees_seen % C::kTrees].bits[node];
-        }
-        const uint4 valid = *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
-        if (nodes || (valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {  // the same for all threads
-          const uint32_t see[4] = {nodes ? path.x : valid.x, nodes ? path.y : valid.y, nodes ? path.z : valid.z,
-                                   nodes ? path.w : valid.w};
+          tc::fence_after_sync();
+          uint32_t x[64];
+          tc::tmem_ld64(ts, x);
+          if (C::kScores < kTile || half == halves - 1) {  // S is in registers: the next one may be written
+            tc::fence_before_sync();
+            __syncwarp();
+            tc::arrive_if(lane == 0, bars.sfree<S>(s));
+          }
+          const uint32_t see0 = half ? see.z : see.x, see1 = half ? see.w : see.y;
+          if (nodes || (see0 & see1) != 0xffffffffu) {  // the same for all threads
 #pragma unroll
-          for (int t = 0; t < 128; ++t)
-            if (!(see[t >> 5] >> (t & 31) & 1u)) x[t] = 0xff800000u;  // -inf
-        }
-        // the row's maximum, its factor and the probabilities
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int t = 0; t < 64; ++t)
+              if (!((t < 32 ? see0 : see1) >> (t & 31) & 1u)) x[t] = 0xff800000u;  // -inf
+          }
+          // the row's maximum, its factor and the probabilities
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int t = 0; t < 128; t += 2) mx[(t >> 1) & 3] = max3(mx[(t >> 1) & 3], __uint_as_float(x[t]), __uint_as_float(x[t + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-        if (j == 0) {
-          m = top;
-        } else {
-          const bool grow = top > m + 8.f || (m == -INFINITY && top != -INFINITY);
+          for (int t = 0; t < 64; t += 2)
+            mx[(t >> 1) & 3] = max3(mx[(t >> 1) & 3], __uint_as_float(x[t]), __uint_as_float(x[t + 1]));
+          const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
+          const bool first = j == 0 && half == 0;
+          const bool grow = first || top > m + 8.f || (m == -INFINITY && top != -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
             const float to_m = grow ? top : m;
-            const float f = grow ? ex2_approx(m - to_m) : 1.f;  // ex2(-inf) = 0: nothing seen before
-            l *= f;
-            m = to_m;
-            // P V of the tile before is complete: S was issued after it
+            if (!first) {
+              const float f = grow ? ex2_approx(m - to_m) : 1.f;  // ex2(-inf) = 0: nothing seen before
+              l *= f;
+              // O is rescaled where it lies, once this stream's P V so far are complete
+              ok = __all_sync(0xffffffffu, wait_phase(bars.pvdone<S>(s), (vc - 1) & 1));
+              if (!ok) break;
+              tc::fence_after_sync();
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tc::tmem_ld16(to + c, o);
 #pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              asm volatile(
-                  "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-                  "tcgen05.wait::ld.sync.aligned;"
-                  : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
-                    "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                  : "r"(to + c)
-                  : "memory");
-#pragma unroll
-              for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
-              tc::tmem_st16(to + c, o);
+                for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+                tc::tmem_st16(to + c, o);
+              }
             }
+            m = to_m;
+            // past 2^20 the fused product below would keep digits that m has lost
+            huge = __any_sync(0xffffffffu, fabsf(m == -INFINITY ? 0.f : m) > 1048576.f);
           }
-        }
-        float ref = m == -INFINITY ? 0.f : m, by = a.scale_log2;
-        // past 2^20 the fused product below would keep digits that m has lost: round it first
-        if (__any_sync(0xffffffffu, fabsf(ref) > 1048576.f)) {
+          float ref = m == -INFINITY ? 0.f : m, by = a.scale_log2;
+          if (huge) {  // the product is rounded first
 #pragma unroll
-          for (int t = 0; t < 128; ++t) x[t] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[t]), by), ref));
-          ref = 0.f;
-          by = 1.f;
-        }
-        const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), minus = pack2(-1.f, -1.f);
-        uint64_t sum[2] = {0, 0};
+            for (int t = 0; t < 64; ++t) x[t] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[t]), by), ref));
+            ref = 0.f;
+            by = 1.f;
+          }
+          const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), minus = pack2(-1.f, -1.f);
+          uint64_t sum[2] = {0, 0};
+          uint32_t hi[32], lo[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
+          for (int q = 0; q < 32; ++q) {
             float p0, p1;
-            unpack2(fma2(pack2(__uint_as_float(x[32 * c + 2 * q]), __uint_as_float(x[32 * c + 2 * q + 1])), by2, ref2), p0, p1);
+            unpack2(fma2(pack2(__uint_as_float(x[2 * q]), __uint_as_float(x[2 * q + 1])), by2, ref2), p0, p1);
             p0 = ex2_approx(p0);
             p1 = ex2_approx(p1);
             const uint64_t p = pack2(p0, p1);
@@ -546,18 +576,26 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             unpack2(fma2(pack2(bf16_lo(hi[q]), bf16_hi(hi[q])), minus, p), p0, p1);
             lo[q] = pack_bf16x2(p0, p1);
           }
-          tc::tmem_st16(ts + 16 * c, hi);
-          tc::tmem_st16(ts + 64 + 16 * c, lo);
-          if (c & 1) {  // a half is there
-            tc::tmem_st_wait();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::arrive(c == 1 ? bars.pfull<S>(s) : bars.plast<S>(s));
+          // the P V before has read P (only one may be under way)
+          if (vc > 0) {
+            ok = __all_sync(0xffffffffu, wait_phase(bars.pvdone<S>(s), (vc - 1) & 1));
+            if (!ok) break;
+            tc::fence_after_sync();
           }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            tc::tmem_st16(tp + 16 * c, hi + 16 * c);
+            tc::tmem_st16(tp + 32 + 16 * c, lo + 16 * c);
+          }
+          tc::tmem_st_wait();
+          tc::fence_before_sync();
+          __syncwarp();
+          tc::arrive_if(lane == 0, bars.pfull<S>(s));
+          ++vc;
+          float s0, s1;
+          unpack2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
         }
-        float s0, s1;
-        unpack2(add2(sum[0], sum[1]), s0, s1);
-        l += s0 + s1;
       }
       if (!ok) break;
       trees_seen += has_tree;
@@ -566,13 +604,13 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       if (next.count > 0) load_q(next, nst);  // every S of this stream is complete: Q may be replaced
       // ---- the segment's result ----
       const bool direct = sg.count == sg.tiles, join = !st.both && st.n[1] > 0;
-      if (n > 0) ok = __all_sync(0xffffffffu, wait_phase(bars.ofull<S>(s), oc++ & 1));
+      if (n > 0) ok = __all_sync(0xffffffffu, wait_phase(bars.pvdone<S>(s), (vc - 1) & 1));
       if (!ok) break;
       if (join && s == 1) {
         other_ml[r] = make_float2(m, l);
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) tc::arrive(bars.other<S>());
+        tc::arrive_if(lane == 0, bars.other<S>());
         // stream 0 reads this stream's O from TMEM before the next segment overwrites it
         ok = __all_sync(0xffffffffu, wait_phase(bars.joined<S>(), jc++ & 1));
         if (!ok) break;
@@ -644,7 +682,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         if (join) {
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) tc::arrive(bars.joined<S>());
+          tc::arrive_if(lane == 0, bars.joined<S>());
         }
       }
       it0 += sg.count;
