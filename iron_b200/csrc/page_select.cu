@@ -1,21 +1,26 @@
 // Decode attention over the pages that a cheap score selects.
 //
-// One kernel; a cluster of CTAs per (sequence, kv head):
+// For few (sequence, kv head) units one kernel, a cluster of CTAs per unit:
 //   1. each CTA scores its share of the pages from their summaries;
 //   2. after a cluster barrier every CTA has all keys (its own and, through distributed
 //      shared memory, the others') and picks the same pages;
 //   3. the kept pages' 16-token blocks are dealt out to the cluster's warps;
 //   4. each CTA merges its warps, and the cluster merges its CTAs, each rank a share of the
 //      output (fixed order throughout).
+// Where the units alone fill the GPU, clusters would run in waves of which the last is
+// partly empty: then steps 1 and 2 are a kernel of their own (one CTA per unit, little
+// shared memory), the kept blocks of all units are cut into as many equal pieces as CTAs
+// run at once, and a third kernel joins the units that were cut.
 // The score is a sum of products of whole numbers: over the heads, q8 meets hi8 where it is
 // positive and lo8 where it is negative, = hi8 . (sum of the positive q8) + lo8 . (sum of
 // the negative q8), so one 16-bit weight vector of 2 D values serves the whole query group,
 // and dp2a (two 16 x 8 bit products per instruction) sums it exactly.
 //
 // Bound: HBM (summaries of all pages, K and V of the kept ones) for batches, the latency of
-// the four steps for single sequences. As four kernels (score, pick, attend, join) the
-// steps of all sequences waited for one another, and 64 sequences of 32768 tokens, 64 pages
-// kept, took 240 us on B200.
+// the four steps for single sequences. B200, 64 sequences of 32768 tokens, 64 pages kept:
+// 240 us with a kernel per step and one block per warp in flight, 141 as clusters, 122 in
+// pieces (with 3 stages in 3 CTAs per SM 8 us more, with 10 in 1 15 more; without any
+// arithmetic on the blocks 10 less).
 #include <cfloat>
 
 #include <cooperative_groups.h>
@@ -38,6 +43,7 @@ struct SelectArgs {
   uint16_t *out;
   int *selected;
   uint32_t *keys;  // workspace [B, Hkv, M] where a sequence's keys do not fit in shared memory, else null
+  float *ws;       // workspace: partials of cut units, two per CTA: O [16][D], then (max, sum) [16]
   int64_t qs[2], os[2];
   int Hq, Hkv, page_shift, M, P, top;
   float scale_log2;
@@ -88,14 +94,89 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 
 template <int D>
 struct SelectCfg {
-  static constexpr int kStages = 3, kCtasPerSm = D == 64 ? 3 : 2;
+  static constexpr int kStages = D == 64 ? 5 : 3, kCtasPerSm = 2;
   static constexpr int kRing = kSWarps * kStages * Stage<D>::kBytes;  // the stages; before them the keys, after them the merge
   static constexpr int kMerge = kSWarps * 16 * D * 4;
   static_assert(kMerge + 16 * (2 + D) * 4 <= kRing, "the merge of the warps and its result fit in the ring");
 };
 
+// Attention of one CTA over blocks first, first + step, ... < blocks (a warp each) of the
+// pages in `kept`: block i lies in page kept[i >> bshift].
 template <int D>
-__global__ void __launch_bounds__(kSThreads, SelectCfg<D>::kCtasPerSm) select_kernel(SelectArgs a) {
+__device__ __forceinline__ void attend_blocks(const SelectArgs &a, WarpAttn<D> &at, Stage<D> *ring, const int2 *kept,
+                                              int len, int h, int first, int step, int blocks) {
+  constexpr int kStages = SelectCfg<D>::kStages;
+  const int bshift = a.page_shift - 4;
+  auto rows = [&](int i, int2 &e) {  // valid tokens of block i
+    e = kept[i >> bshift];
+    const int in = min(16, len - (e.x << a.page_shift) - ((i & ((1 << bshift) - 1)) << 4));
+    return e.y >= 0 && e.y < a.P ? in : 0;
+  };
+  auto request = [&](int i, int stage) {
+    if (i < blocks) {
+      int2 e;
+      const int valid = rows(i, e);
+      const int64_t at0 = valid > 0 ? (((static_cast<int64_t>(e.y) * a.Hkv + h) << a.page_shift) +
+                                       ((i & ((1 << bshift) - 1)) << 4)) * D : 0;
+      ring[stage].load(a.k + at0, a.v + at0, D, D, valid);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) request(first + s * step, s);
+  int stage = 0;
+  for (int i = first; i < blocks; i += step) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();  // the block is here, and every lane is done with the stage refilled next
+    request(i + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    int2 e;
+    const int valid = rows(i, e);
+    if (valid > 0) {
+      const uint32_t see[2] = {0xffffu >> (16 - valid), 0xffffu >> (16 - valid)};
+      at.step(ring[stage], a.scale_log2, see);
+    }
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+  at.finish();
+}
+
+// The warps' results into shared memory; merged<D>(r, d) is then the CTA's.
+template <int D>
+struct WarpMerge {
+  float (*o)[16][D];
+  float (*m)[16], (*l)[16];
+  __device__ __forceinline__ void put(const WarpAttn<D> &at) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
+    if (tid == 0) {
+      m[warp][gid] = at.m[0];
+      m[warp][gid + 8] = at.m[1];
+      l[warp][gid] = at.l[0];
+      l[warp][gid + 8] = at.l[1];
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      *reinterpret_cast<float2 *>(&o[warp][gid][8 * j + 2 * tid]) = make_float2(at.o[j][0], at.o[j][1]);
+      *reinterpret_cast<float2 *>(&o[warp][gid + 8][8 * j + 2 * tid]) = make_float2(at.o[j][2], at.o[j][3]);
+    }
+  }
+  __device__ __forceinline__ void get(int r, int d, float &M, float &L, float &O) const {
+    M = -INFINITY;
+    L = O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSWarps; ++w) M = fmaxf(M, m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kSWarps; ++w) {
+      const float f = rescale(m[w][r], M);
+      L += l[w][r] * f;
+      O += o[w][r][d] * f;
+    }
+  }
+};
+
+// kAttend: all four steps; else the choice alone (its list goes to `selected`).
+template <int D, bool kAttend>
+__global__ void __launch_bounds__(kSThreads, kAttend ? SelectCfg<D>::kCtasPerSm : 4) select_kernel(SelectArgs a) {
   using C = SelectCfg<D>;
   constexpr int kStages = C::kStages;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -291,86 +372,40 @@ __global__ void __launch_bounds__(kSThreads, SelectCfg<D>::kCtasPerSm) select_ke
       const int k = kind(i);
       if (k == 2 || (k == 1 && v.y < left)) {
         const int to = v.x + min(v.y, left);
-        kept[to] = make_int2(i, ld_act_i32(table + i));
+        if constexpr (kAttend) kept[to] = make_int2(i, ld_act_i32(table + i));
         if (rank == 0) sel[to] = i;
       }
       v.x += k == 2;
       v.y += k == 1;
     }
-    // no CTA may reuse its keys (the ring) while another one copies them
+    // no CTA may reuse its keys (the ring), or leave, while another one copies them
     meet();
   } else {
     for (int i = threadIdx.x; i < a.top; i += kSThreads) {
-      if (i < n) kept[i] = make_int2(i, ld_act_i32(table + i));
+      if constexpr (kAttend)
+        if (i < n) kept[i] = make_int2(i, ld_act_i32(table + i));
       if (rank == 0) sel[i] = i < n ? i : -1;
     }
     __syncthreads();
   }
 
+  if constexpr (!kAttend) return;
+
   // ---- 3. attention over the kept pages' blocks: block i to warp i % (ranks * kSWarps) ----
   WarpAttn<D> at;
   at.clear();
   at.load_q(gid < g ? q + gid * a.qs[1] : nullptr, gid + 8 < g ? q + (gid + 8) * a.qs[1] : nullptr);
-  const int bshift = a.page_shift - 4, blocks = count << bshift, step = ranks * kSWarps;
-  auto rows = [&](int i, int2 &e) {  // valid tokens of block i
-    e = kept[i >> bshift];
-    const int in = min(16, len - (e.x << a.page_shift) - ((i & ((1 << bshift) - 1)) << 4));
-    return e.y >= 0 && e.y < a.P ? in : 0;
-  };
-  auto request = [&](int i, int stage) {
-    if (i < blocks) {
-      int2 e;
-      const int valid = rows(i, e);
-      const int64_t at0 = valid > 0 ? (((static_cast<int64_t>(e.y) * a.Hkv + h) << a.page_shift) +
-                                       ((i & ((1 << bshift) - 1)) << 4)) * D : 0;
-      ring[stage].load(a.k + at0, a.v + at0, D, D, valid);
-    }
-    cp_async_commit();
-  };
-  const int first = rank * kSWarps + warp;
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) request(first + s * step, s);
-  int stage = 0;
-  for (int i = first; i < blocks; i += step) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();  // the block is here, and every lane is done with the stage refilled next
-    request(i + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
-    int2 e;
-    const int valid = rows(i, e);
-    if (valid > 0) {
-      const uint32_t see[2] = {0xffffu >> (16 - valid), 0xffffu >> (16 - valid)};
-      at.step(ring[stage], a.scale_log2, see);
-    }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-  }
-  cp_async_wait<0>();
-  at.finish();
+  attend_blocks<D>(a, at, ring, kept, len, h, rank * kSWarps + warp, ranks * kSWarps, count << (a.page_shift - 4));
   __syncthreads();  // every warp is done with the ring
 
   // ---- 4. the warps of this CTA, then the CTAs of the cluster ----
-  if (tid == 0) {
-    red_m[warp][gid] = at.m[0];
-    red_m[warp][gid + 8] = at.m[1];
-    red_l[warp][gid] = at.l[0];
-    red_l[warp][gid + 8] = at.l[1];
-  }
-#pragma unroll
-  for (int j = 0; j < D / 8; ++j) {
-    *reinterpret_cast<float2 *>(&red_o[warp][gid][8 * j + 2 * tid]) = make_float2(at.o[j][0], at.o[j][1]);
-    *reinterpret_cast<float2 *>(&red_o[warp][gid + 8][8 * j + 2 * tid]) = make_float2(at.o[j][2], at.o[j][3]);
-  }
+  WarpMerge<D> merge{red_o, red_m, red_l};
+  merge.put(at);
   __syncthreads();
   for (int idx = threadIdx.x; idx < g * D; idx += kSThreads) {
     const int r = idx / D, d = idx % D;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll
-    for (int w = 0; w < kSWarps; ++w) M = fmaxf(M, red_m[w][r]);
-#pragma unroll
-    for (int w = 0; w < kSWarps; ++w) {
-      const float f = rescale(red_m[w][r], M);
-      L += red_l[w][r] * f;
-      O += red_o[w][r][d] * f;
-    }
+    float M, L, O;
+    merge.get(r, d, M, L, O);
     if (d == 0) {
       part[r][0] = M;
       part[r][1] = L;
@@ -406,6 +441,104 @@ __global__ void __launch_bounds__(kSThreads, SelectCfg<D>::kCtasPerSm) select_ke
   meet();  // no CTA leaves while another one reads its part
 }
 
+// Pieces: `per` blocks per unit (those past a unit's own do nothing), cut into gridDim.x
+// equal parts.
+template <int D>
+__global__ void __launch_bounds__(kSThreads, SelectCfg<D>::kCtasPerSm) select_attend_kernel(SelectArgs a, int units, int per) {
+  using C = SelectCfg<D>;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  Stage<D> *ring = reinterpret_cast<Stage<D> *>(dyn) + (threadIdx.x >> 5) * C::kStages;
+  int2 *kept = reinterpret_cast<int2 *>(dyn + C::kRing);
+  __shared__ float red_m[kSWarps][16], red_l[kSWarps][16];
+  WarpMerge<D> merge{reinterpret_cast<float (*)[16][D]>(dyn), red_m, red_l};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, g = a.Hq / a.Hkv, bshift = a.page_shift - 4;
+  const int64_t total = static_cast<int64_t>(units) * per;
+  int64_t w = total * blockIdx.x / gridDim.x;
+  const int64_t w_end = total * (blockIdx.x + 1) / gridDim.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  while (w < w_end) {
+    const int unit = static_cast<int>(w / per), b0 = static_cast<int>(w % per);
+    const int b1 = static_cast<int>(min(static_cast<int64_t>(per), b0 + (w_end - w)));
+    w += b1 - b0;
+    const int h = unit % a.Hkv, b = unit / a.Hkv;
+    const int len = cached_len(a, b), n = (len + (1 << a.page_shift) - 1) >> a.page_shift;
+    const int blocks = min(b1, min(n, a.top) << bshift);
+    const int *sel = a.selected + static_cast<int64_t>(unit) * a.top, *table = a.table + static_cast<int64_t>(b) * a.M;
+    for (int i = (b0 >> bshift) + threadIdx.x; i < (blocks + (1 << bshift) - 1) >> bshift; i += kSThreads) {
+      const int at = ld_act_i32(sel + i);
+      kept[i] = make_int2(at, ld_act_i32(table + at));
+    }
+    const uint16_t *q = a.q + b * a.qs[0] + static_cast<int64_t>(h) * g * a.qs[1];
+    WarpAttn<D> at;
+    at.clear();
+    at.load_q(gid < g ? q + gid * a.qs[1] : nullptr, gid + 8 < g ? q + (gid + 8) * a.qs[1] : nullptr);
+    __syncthreads();  // the list is there, and the merge before is done with the ring
+    attend_blocks<D>(a, at, ring, kept, len, h, b0 + warp, kSWarps, blocks);
+    __syncthreads();
+    merge.put(at);
+    __syncthreads();
+    const bool whole = b0 == 0 && b1 == per;
+    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (b0 == 0 ? 1 : 0)) * 16 * (D + 2);
+    for (int idx = threadIdx.x; idx < g * D; idx += kSThreads) {
+      const int r = idx / D, d = idx % D;
+      float M, L, O;
+      merge.get(r, d, M, L, O);
+      if (whole) {
+        a.out[b * a.os[0] + (static_cast<int64_t>(h) * g + r) * a.os[1] + d] = float_to_bf16_bits(normalised(O, L));
+      } else {
+        if (d == 0) {
+          part[16 * D + 2 * r] = M;
+          part[16 * D + 2 * r + 1] = L;
+        }
+        part[r * D + d] = O;
+      }
+    }
+    __syncthreads();  // kept and the merge may be used again
+  }
+}
+
+// Joins the pieces of one unit, in order; a unit that one piece held whole has none.
+template <int D>
+__global__ void __launch_bounds__(256) select_join_kernel(SelectArgs a, int units, int per, int pieces) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int unit = blockIdx.x, h = unit % a.Hkv, b = unit / a.Hkv, g = a.Hq / a.Hkv;
+  const int64_t total = static_cast<int64_t>(units) * per, w = static_cast<int64_t>(unit) * per;
+  const int c0 = static_cast<int>(((w + 1) * pieces - 1) / total), c1 = static_cast<int>(((w + per) * pieces - 1) / total);
+  if (c0 == c1) return;
+  for (int idx = threadIdx.x; idx < g * D; idx += 256) {
+    const int r = idx / D, d = idx % D;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+    for (int c = c0; c <= c1; c += 4) {
+      float2 ml[4];
+      float o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = c + i <= c1;
+        const float *part = a.ws + (static_cast<int64_t>(in ? c + i : c0) * 2 + (c + i == c0 || !in ? 1 : 0)) * 16 * (D + 2);
+        ml[i] = __ldcg(reinterpret_cast<const float2 *>(part + 16 * D + 2 * r));
+        o[i] = __ldcg(part + r * D + d);
+        if (!in) ml[i] = make_float2(-INFINITY, 0.f), o[i] = 0.f;
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+      const float f0 = rescale(M, top);
+      M = top;
+      L *= f0;
+      O *= f0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = rescale(ml[i].x, M);
+        L += ml[i].y * f;
+        O += o[i] * f;
+      }
+    }
+    a.out[b * a.os[0] + (static_cast<int64_t>(h) * g + r) * a.os[1] + d] = float_to_bf16_bits(normalised(O, L));
+  }
+}
+
 }  // namespace iron
 
 using namespace iron;
@@ -415,32 +548,51 @@ static bool keys_in_workspace(int head_dim, int max_pages) {
   return static_cast<int64_t>(max_pages) * 4 > (head_dim == 128 ? SelectCfg<128>::kRing : SelectCfg<64>::kRing);
 }
 
-// CTAs of a (sequence, kv head): clusters as large as leave every warp a block of the kept
-// pages, while all CTAs run at once (what is done once per CTA takes as long as some 100 KB
-// of pages: at 16 sequences, head dim 128, clusters of 2 took 60 us, of 8 89 us on B200).
-static int select_ranks(int units, int top, int page, int ctas_per_sm) {
-  const int64_t blocks = static_cast<int64_t>(top) * page / 16;
-  int r = 16;
-  while (r > 1 && (static_cast<int64_t>(units) * r > static_cast<int64_t>(ctas_per_sm) * sm_count() || blocks < r * kSWarps)) r /= 2;
-  return r;
+// CTAs of a (sequence, kv head). Time goes in waves of CTAs that run at once; each takes what
+// is done once per CTA -- about as long as 190 KB of its share of the memory's bandwidth --
+// and its part of the pages. The cluster size of the least waves x time is taken, as far
+// as every warp gets a block. B200: 16 sequences of 32768 tokens at head dim 128 (128
+// units, 296 CTAs at once), 32 pages of 64 tokens: 1 CTA 61 us, 2 41, 4 53; 1 sequence,
+// 16 pages: 1 17 us, 4 12, 16 13.
+static int select_ranks(int64_t units, int top, int page, int head_dim, int max_pages, int ctas) {
+  const int64_t blocks = static_cast<int64_t>(top < max_pages ? top : max_pages) * page / 16;
+  const int64_t bytes = blocks * 16 * head_dim * 4 + static_cast<int64_t>(max_pages) * (2 * head_dim + 4);
+  int best = 1;
+  int64_t least = 0;
+  for (int r = 1; r <= 16 && (r == 1 || blocks >= r * kSWarps); r *= 2) {
+    const int64_t cost = ((units * r + ctas - 1) / ctas) * (190 * 1024 + bytes / r);
+    if (r == 1 || cost < least) {
+      best = r;
+      least = cost;
+    }
+  }
+  return best;
 }
+
+// Whether the units alone fill the GPU, so that the kept blocks are cut into pieces.
+static bool in_pieces(int64_t units, int ctas) { return 2 * units > ctas; }
 
 template <int D>
 static int launch_select(const SelectArgs &a, int B, int page, cudaStream_t s) {
-  const int ranks = select_ranks(B * a.Hkv, a.top, page, SelectCfg<D>::kCtasPerSm);
-  const int list = (a.top < a.M ? a.top : a.M) * static_cast<int>(sizeof(int2));
+  using C = SelectCfg<D>;
+  const int ctas = C::kCtasPerSm * sm_count(), units = B * a.Hkv, longest = a.top < a.M ? a.top : a.M;
+  const bool pieces = in_pieces(units, ctas);
+  const int ranks = pieces ? 1 : select_ranks(units, a.top, page, D, a.M, ctas);
+  const int list = longest * static_cast<int>(sizeof(int2));
   static PerDeviceOnce once;
   const int st = once.run([] {
-    cudaError_t e = cudaFuncSetAttribute(select_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         SelectCfg<D>::kRing + kMaxTop * static_cast<int>(sizeof(int2)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(select_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const int most = C::kRing + kMaxTop * static_cast<int>(sizeof(int2));
+    cudaError_t e = cudaFuncSetAttribute(select_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(select_kernel<D, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(select_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(select_attend_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     return call_status(e);
   });
   if (st != IRON_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(B * a.Hkv * ranks);
+  cfg.gridDim = dim3(units * ranks);
   cfg.blockDim = dim3(kSThreads);
-  cfg.dynamicSmemBytes = SelectCfg<D>::kRing + list;
+  cfg.dynamicSmemBytes = pieces ? (a.keys ? 0 : a.M * sizeof(uint32_t)) : static_cast<size_t>(C::kRing + list);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -450,13 +602,28 @@ static int launch_select(const SelectArgs &a, int B, int page, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return call_status(cudaLaunchKernelEx(&cfg, select_kernel<D>, a));
+  if (!pieces) return call_status(cudaLaunchKernelEx(&cfg, select_kernel<D, true>, a));
+  int e = call_status(cudaLaunchKernelEx(&cfg, select_kernel<D, false>, a));
+  if (e != IRON_OK) return e;
+  const int per = longest * (page / 16);
+  const int64_t total = static_cast<int64_t>(units) * per;
+  const int grid = static_cast<int>(total < ctas ? total : ctas);
+  e = launch(select_attend_kernel<D>, dim3(grid), dim3(kSThreads), C::kRing + list, s, true, a, units, per);
+  if (e != IRON_OK) return e;
+  return launch(select_join_kernel<D>, dim3(units), dim3(256), 0, s, true, a, units, per, grid);
+}
+
+// The workspace: partials of cut units, then the keys that do not fit in shared memory.
+static size_t select_partials(int64_t units, int head_dim) {
+  const int ctas = (head_dim == 128 ? SelectCfg<128>::kCtasPerSm : SelectCfg<64>::kCtasPerSm) * sm_count();
+  return in_pieces(units, ctas) ? static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2) * sizeof(float) : 0;
 }
 
 extern "C" size_t iron_page_select_attn_workspace_bytes(int batch, int num_heads, int kv_heads, int head_dim,
                                                         int max_pages, int top_pages, int page_size) {
   if (batch <= 0 || num_heads <= 0 || kv_heads <= 0 || max_pages <= 0 || top_pages <= 0 || page_size <= 0) return 0;
-  return keys_in_workspace(head_dim, max_pages) ? static_cast<size_t>(batch) * kv_heads * max_pages * 4 : 16;
+  return 16 + select_partials(static_cast<int64_t>(batch) * kv_heads, head_dim) +
+         (keys_in_workspace(head_dim, max_pages) ? static_cast<size_t>(batch) * kv_heads * max_pages * 4 : 0);
 }
 
 extern "C" int iron_page_select_attn(const iron_page_pool *c, const uint16_t *q, uint16_t *out, int32_t *selected,
@@ -470,7 +637,7 @@ extern "C" int iron_page_select_attn(const iron_page_pool *c, const uint16_t *q,
   if (c->layers != 1 || num_heads <= 0 || num_heads % c->kv_heads || top_pages <= 0) return IRON_ERR_SHAPE;
   if (c->slots > 65535) return IRON_ERR_SHAPE;
   if (num_heads / c->kv_heads > 16 || top_pages > kMaxTop) return IRON_ERR_UNSUPPORTED;
-  if (!aligned16(q)) return IRON_ERR_ALIGN;
+  if (!aligned16(q) || !aligned16(workspace)) return IRON_ERR_ALIGN;
   for (int i = 0; i < 2; ++i)
     if (q_strides[i] % 8 || out_strides[i] % 8) return IRON_ERR_ALIGN;
   if (workspace_bytes < iron_page_select_attn_workspace_bytes(c->slots, num_heads, c->kv_heads, c->head_dim,
@@ -486,7 +653,11 @@ extern "C" int iron_page_select_attn(const iron_page_pool *c, const uint16_t *q,
   a.lens = c->lens;
   a.out = out;
   a.selected = selected;
-  a.keys = keys_in_workspace(c->head_dim, c->max_pages) ? static_cast<uint32_t *>(workspace) : nullptr;
+  a.ws = static_cast<float *>(workspace);
+  a.keys = keys_in_workspace(c->head_dim, c->max_pages)
+               ? reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(workspace) +
+                                              select_partials(static_cast<int64_t>(c->slots) * c->kv_heads, c->head_dim))
+               : nullptr;
   for (int i = 0; i < 2; ++i) {
     a.qs[i] = q_strides[i];
     a.os[i] = out_strides[i];
