@@ -482,7 +482,9 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * its values. q, out bf16 [batch, num_nodes, Hq, D], k_new, v_new bf16 [batch, num_nodes,
  * kv_heads, D] with element strides {batch, node, head} (3 int64 each, multiples of 8; kv
  * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024.
- * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split.
+ * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split, and
+ * counters: it must be zero before its first use; calls leave them zero (one workspace
+ * may serve calls of the same sizes that do not overlap on the GPU).
  * From 33 rows (nodes x Hq / kv_heads) per kv head on it runs on the tcgen05 tensor cores;
  * iron_tree_attn_status returns IRON_ERR_TIMEOUT if a bounded wait ran out there since the
  * last reset (reset != 0 clears it); it synchronises the device. */

@@ -13,6 +13,8 @@ that of ``iron_page_pool`` in include/iron_b200.h:
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 
 from .. import _lib
@@ -48,7 +50,7 @@ class PagedOperator(MLIROperator):
         if ws is None:
             import torch
 
-            t = torch.empty(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
+            t = torch.zeros(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
             ws = self._spaces[stream] = (t.data_ptr(), t.numel(), t)
         return ws[0], ws[1]
 
@@ -110,6 +112,17 @@ def address(t):
     if not t.is_cuda:
         raise RuntimeError("iron_b200 kernels take CUDA tensors; got a host tensor")
     return t.data_ptr()
+
+
+_stride_arrays: dict = {}
+
+
+def stride_array(strides):
+    """The strides as an int64 array for the C entry points (made once per set of strides)."""
+    a = _stride_arrays.get(strides)
+    if a is None:
+        a = _stride_arrays[strides] = (ctypes.c_int64 * len(strides))(*strides)
+    return a
 
 
 def strides(t, shape):

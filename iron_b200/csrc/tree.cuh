@@ -13,7 +13,8 @@ struct TreeArgs {
   const uint16_t *q, *k_new, *v_new, *k, *v;
   const int *table, *lens, *parents;
   uint16_t *out;
-  float *ws;  // partials: what a piece of the work leaves of a unit that it holds in part
+  float *ws;         // partials: what a piece of the work leaves of a unit that it holds in part
+  unsigned *counts;  // pieces of a unit that are done (0 between calls)
   int64_t qs[3], ks[3], os[3];  // element strides {batch, node, head}
   int B, N, Hq, Hkv, groups /* row groups per (sequence, kv head) */, page_shift, M, P;
   float scale_log2;

@@ -26,10 +26,8 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, address, strides
+from ...common.paged import PagedOperator, address, stride_array, strides
 from ...common.verify import Tolerance
-
-_I64x2 = ctypes.c_int64 * 2
 
 
 @dataclass
@@ -79,7 +77,7 @@ class PageSelectAttention(PagedOperator):
                              self.num_pages, self.max_pages, self.num_kv_heads, self.head_dim, self.page_size)
         scale = 1.0 / math.sqrt(self.head_dim) if self.scale is None else self.scale
         _lib.call("iron_page_select_attn", ctypes.byref(pool), p(q), p(out), p(selected), self.num_heads,
-                  self.top_pages, _I64x2(*strides(q, rows)), _I64x2(*strides(out, rows)), scale, ws, nbytes, flags, stream)
+                  self.top_pages, stride_array(strides(q, rows)), stride_array(strides(out, rows)), scale, ws, nbytes, flags, stream)
 
     def reference(self, q, k_pages, v_pages, codes, scales, page_table, lens):
         """(out, selected) by the rule, head by head."""

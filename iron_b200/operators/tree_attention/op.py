@@ -27,10 +27,8 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, address, strides
+from ...common.paged import PagedOperator, address, stride_array, strides
 from ...common.verify import Tolerance
-
-_I64x3 = ctypes.c_int64 * 3
 
 
 @dataclass
@@ -84,7 +82,7 @@ class TreeAttention(PagedOperator):
                              self.num_pages, self.max_pages, self.num_kv_heads, self.head_dim, self.page_size)
         scale = 1.0 / math.sqrt(self.head_dim) if self.scale is None else self.scale
         _lib.call("iron_tree_attn", ctypes.byref(pool), p(q), p(k_new), p(v_new), p(parents), p(out), self.num_nodes,
-                  self.num_heads, _I64x3(*strides(q, rows)), _I64x3(*ks), _I64x3(*strides(out, rows)), scale, ws,
+                  self.num_heads, stride_array(strides(q, rows)), stride_array(ks), stride_array(strides(out, rows)), scale, ws,
                   nbytes, flags, stream)
 
     def reference(self, q, k_new, v_new, k_pages, v_pages, page_table, lens, parents):
