@@ -100,6 +100,13 @@ def test_wide_table_and_ragged_batch():
     run([9000, 1, 300], 60, 8, 1, 128, 64, seed=4, width=2000)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [3, 20, 64])
+def test_many_tiles_per_piece(N, D):
+    """More tiles than the GPU has CTAs: pieces of many tiles, and of several sequences."""
+    run([4096, 2999, 2049, 100, 3100, 0, 4000, 640], N, 32, 8, D, 64, seed=N)
+
+
 def test_batch_of_many():
     rng = random.Random(2)
     run([rng.randint(0, 200) for _ in range(300)], 2, 4, 1, 64, 32, seed=2)
