@@ -7,8 +7,8 @@
 //   3. the kept pages' 16-token blocks are dealt out to the cluster's warps;
 //   4. each CTA merges its warps, and the cluster merges its CTAs, each rank a share of the
 //      output (fixed order throughout).
-// Where the units alone fill the GPU, clusters would run in waves of which the last is
-// partly empty: then steps 1 and 2 are a kernel of their own (one CTA per unit, little
+// With more units clusters run in waves of which the last is partly empty. Where that costs
+// more than two further launches, steps 1 and 2 are a kernel of their own (one CTA per unit, little
 // shared memory), the kept blocks of all units are cut into as many equal pieces as CTAs
 // run at once, and a third kernel joins the units that were cut.
 // The score is a sum of products of whole numbers: over the heads, q8 meets hi8 where it is
@@ -548,36 +548,43 @@ static bool keys_in_workspace(int head_dim, int max_pages) {
   return static_cast<int64_t>(max_pages) * 4 > (head_dim == 128 ? SelectCfg<128>::kRing : SelectCfg<64>::kRing);
 }
 
-// CTAs of a (sequence, kv head). Time goes in waves of CTAs that run at once; each takes what
-// is done once per CTA -- about as long as 190 KB of its share of the memory's bandwidth --
-// and its part of the pages. The cluster size of the least waves x time is taken, as far
-// as every warp gets a block. B200: 16 sequences of 32768 tokens at head dim 128 (128
-// units, 296 CTAs at once), 32 pages of 64 tokens: 1 CTA 61 us, 2 41, 4 53; 1 sequence,
-// 16 pages: 1 17 us, 4 12, 16 13.
-static int select_ranks(int64_t units, int top, int page, int head_dim, int max_pages, int ctas) {
+// The form with the least time, in bytes that a CTA could move meanwhile at its share of the
+// memory's bandwidth (48 us per MB; summaries go at half of it). Clusters go in waves of
+// CTAs that run at once; each CTA takes 190 KB for what is done once per CTA, 5 KB more per
+// rank that it meets, and its part of the unit's bytes. Clusters of 16 leave about a quarter
+// of the SMs idle. Pieces take 450 KB for three kernels and the joins, a unit's summaries
+// in one CTA, twice as slowly (nothing else runs), and an even share of all pages. B200, us,
+// pieces / clusters: 32768 tokens, 64 pages of 64, head dim 64: 128 units 48 / 42, 152
+// 53 / 62, 256 73 / 68, 384 97 / 116, 512 121 / 128; head dim 128, 32 pages: 64 units 44 / 27,
+// 152 75 / 65, 256 94 / 79, 384 118 / 128, 512 139 / 142; 8192 tokens, 16 pages: 256 units
+// 27 / 22, 384 35 / 43. Cluster sizes: 128 units of 32768 tokens, 32 pages, head dim 128: 1 CTA
+// 61, 2 41, 4 53; 8 units of 8192 tokens, 16 pages: 1 CTA 17, 8 11.9, 16 12.6; 16 units, 1024
+// pages: 8 CTAs 105, 16 121.
+struct SelectPlan {
+  bool pieces;
+  int ranks;  // CTAs of a unit's cluster
+};
+static SelectPlan select_plan(int64_t units, int top, int page, int head_dim, int max_pages, int ctas) {
   const int64_t blocks = static_cast<int64_t>(top < max_pages ? top : max_pages) * page / 16;
-  const int64_t bytes = blocks * 16 * head_dim * 4 + static_cast<int64_t>(max_pages) * (2 * head_dim + 4);
-  int best = 1;
-  int64_t least = 0;
+  const int64_t pages = blocks * 16 * head_dim * 4, summaries = static_cast<int64_t>(max_pages) * (2 * head_dim + 4);
+  SelectPlan best = {true, 1};
+  int64_t least = 450 * 1024 + (units > ctas ? summaries * units / ctas : summaries) + 3 * summaries + pages * units / ctas;
   for (int r = 1; r <= 16 && (r == 1 || blocks >= r * kSWarps); r *= 2) {
-    const int64_t cost = ((units * r + ctas - 1) / ctas) * (190 * 1024 + bytes / r);
-    if (r == 1 || cost < least) {
-      best = r;
+    const int fit = r == 16 ? ctas * 3 / 4 : ctas;
+    const int64_t cost = ((units * r + fit - 1) / fit) * (190 * 1024 + 5 * 1024 * r + (pages + 2 * summaries) / r);
+    if (cost < least) {
+      best = {false, r};
       least = cost;
     }
   }
   return best;
 }
 
-// Whether the units alone fill the GPU, so that the kept blocks are cut into pieces.
-static bool in_pieces(int64_t units, int ctas) { return 2 * units > ctas; }
-
 template <int D>
 static int launch_select(const SelectArgs &a, int B, int page, cudaStream_t s) {
   using C = SelectCfg<D>;
   const int ctas = C::kCtasPerSm * sm_count(), units = B * a.Hkv, longest = a.top < a.M ? a.top : a.M;
-  const bool pieces = in_pieces(units, ctas);
-  const int ranks = pieces ? 1 : select_ranks(units, a.top, page, D, a.M, ctas);
+  const auto [pieces, ranks] = select_plan(units, a.top, page, D, a.M, ctas);
   const int list = longest * static_cast<int>(sizeof(int2));
   static PerDeviceOnce once;
   const int st = once.run([] {
@@ -614,15 +621,17 @@ static int launch_select(const SelectArgs &a, int B, int page, cudaStream_t s) {
 }
 
 // The workspace: partials of cut units, then the keys that do not fit in shared memory.
-static size_t select_partials(int64_t units, int head_dim) {
+static size_t select_partials(int64_t units, int top, int page, int head_dim, int max_pages) {
   const int ctas = (head_dim == 128 ? SelectCfg<128>::kCtasPerSm : SelectCfg<64>::kCtasPerSm) * sm_count();
-  return in_pieces(units, ctas) ? static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2) * sizeof(float) : 0;
+  return select_plan(units, top, page, head_dim, max_pages, ctas).pieces
+             ? static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2) * sizeof(float)
+             : 0;
 }
 
 extern "C" size_t iron_page_select_attn_workspace_bytes(int batch, int num_heads, int kv_heads, int head_dim,
                                                         int max_pages, int top_pages, int page_size) {
   if (batch <= 0 || num_heads <= 0 || kv_heads <= 0 || max_pages <= 0 || top_pages <= 0 || page_size <= 0) return 0;
-  return 16 + select_partials(static_cast<int64_t>(batch) * kv_heads, head_dim) +
+  return 16 + select_partials(static_cast<int64_t>(batch) * kv_heads, top_pages, page_size, head_dim, max_pages) +
          (keys_in_workspace(head_dim, max_pages) ? static_cast<size_t>(batch) * kv_heads * max_pages * 4 : 0);
 }
 
@@ -656,7 +665,8 @@ extern "C" int iron_page_select_attn(const iron_page_pool *c, const uint16_t *q,
   a.ws = static_cast<float *>(workspace);
   a.keys = keys_in_workspace(c->head_dim, c->max_pages)
                ? reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(workspace) +
-                                              select_partials(static_cast<int64_t>(c->slots) * c->kv_heads, c->head_dim))
+                                              select_partials(static_cast<int64_t>(c->slots) * c->kv_heads, top_pages,
+                                                              c->page_size, c->head_dim, c->max_pages))
                : nullptr;
   for (int i = 0; i < 2; ++i) {
     a.qs[i] = q_strides[i];

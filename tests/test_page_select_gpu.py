@@ -185,3 +185,17 @@ def test_operator_reference_agrees():
     op = PageSelectAttention(batch=3, num_heads=8, num_kv_heads=2, head_dim=64, page_size=16, num_pages=cache.P, max_pages=cache.M, top_pages=4)
     out, sel = op.reference(*(t.cpu() for t in (q, cache.k, cache.v, codes, scales, cache.table, cache.lens)))
     check(cache, q, codes, scales, 4, out.cuda(), sel.cuda())
+
+
+@pytest.mark.parametrize("D,pages", [(64, 23500), (128, 26200)])
+def test_more_pages_than_keys_fit(D, pages):
+    """Sequences whose scores do not fit in shared memory; the second one is short."""
+    run([pages * 16 - 11, 100, 0], 40, 8, 2, D, 16, seed=D, width=pages + 3)
+
+
+@pytest.mark.parametrize("D,width", [(64, None), (128, None), (64, 23500), (128, 26200)])
+def test_more_units_than_ctas(D, width):
+    """300 (sequence, kv head) units of all lengths: pieces that hold parts of several."""
+    rng = random.Random(D)
+    lens = [rng.choice([0, 1, 63, 64, 65, 700, 2048, 3000]) for _ in range(150)]
+    run(lens, 20, 8, 2, D, 64, seed=D + 1, width=width)
