@@ -1,8 +1,8 @@
 // Attention of a tree of drafted tokens over a paged KV cache.
 //
 // Rows: the Hq / Hkv query heads of all nodes share a kv head, so a (sequence, kv head)
-// has num_nodes * group rows that read the same cached K and V. They are cut into groups
-// of 16 rows (the M of mma.sync m16n8k16). Work: every unit = (sequence, kv head, row
+// has num_nodes * group rows that read the same cached K and V. They are cut into groups of
+// 16 or 32 rows (mma.sync m16n8k16 has 16). Work: every unit = (sequence, kv head, row
 // group) is a list of 64-token tiles -- the cached ones, then the tree's own nodes -- and
 // the concatenation of all units' tiles is cut into as many equal pieces as CTAs fit on
 // the GPU. Lengths are read on the device, so ragged batches and tables wider than the
@@ -14,45 +14,52 @@
 
 namespace iron {
 
-constexpr int kTRows = 16;     // rows per unit
 constexpr int kTTile = 64;     // tokens per tile: 16 per warp
 constexpr int kTWarps = 4;
 struct TreeCut {
   static constexpr int kTile = kTTile, kUnitCost = 1;
 };
 
-template <int D>
+// kM: groups of 16 rows that a warp holds, and a unit has.
+template <int D, int kM>
 struct TreeCfg {
-  static constexpr int kStages = 3, kCtasPerSm = D == 64 ? 3 : 2;
+  static constexpr int kStages = 3, kCtasPerSm = D == 64 && kM == 1 ? 3 : 2, kRows = 16 * kM;
+  static constexpr int kPart = kRows * (2 + D);  // floats of a partial: O, then (m, l)
   static constexpr int kRing = kTWarps * kStages * Stage<D>::kBytes;  // the stages; after them the merge
-  static constexpr int kMerge = kTWarps * kTRows * D * 4;
+  static constexpr int kMerge = kTWarps * kRows * D * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
-// Joins the partials of one unit (pieces c0 .. c1), in the order of its tiles, by one CTA; a
-// thread owns 4 values of a row. kJoin pieces are loaded at a time, so a unit of many
-// pieces costs a memory round trip per kJoin of them.
+// Joins partials of one unit, those of pieces first, first + step, ... <= last, in the order
+// of its tiles, by one CTA; a thread owns 4 values of a row. kJoin of them are loaded at a
+// time, so the join takes a memory round trip per kJoin. A unit of more than 2 kJoin pieces
+// is joined in two steps (B200, one sequence of 4608 tokens, 4 nodes: 24.5 -> 14.5 us; with
+// 10 to 14 pieces per unit two steps take 1 us more than one): each kJoin pieces by the
+// last of them to finish, which leaves the result in the place of the first's, then those
+// by the last of all (`to`: that place; null: the output).
 constexpr int kJoin = 8;
 
-template <int D>
-__device__ __forceinline__ void join_unit(const TreeArgs &a, int b, int h, int row0, int c0, int c1) {
+template <int D, int kM>
+__device__ __forceinline__ void join(const TreeArgs &a, int b, int h, int row0, int c0, int first, int last, int step, float *to) {
+  using C = TreeCfg<D, kM>;
   const int g = a.Hq / a.Hkv;
-#pragma unroll 2
-  for (int idx = threadIdx.x; idx < kTRows * D / 4; idx += 32 * kTWarps) {
-    const int r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
-    if (row >= a.N * g) break;
+  for (int idx0 = 0; idx0 < C::kRows * D / 4; idx0 += 32 * kTWarps) {
+    const int idx = idx0 + threadIdx.x, r = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + r;
+    const bool in_rows = row < a.N * g;
     float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
     bool dead = false;
-    for (int c = c0; c <= c1; c += kJoin) {
+    for (int c = first; c <= last && in_rows; c += kJoin * step) {
       float2 ml[kJoin];
       float4 o[kJoin];
 #pragma unroll
       for (int i = 0; i < kJoin; ++i) {
-        const bool in = c + i <= c1;
-        const float *part = a.ws + (static_cast<int64_t>(in ? c + i : c0) * 2 + (c + i == c0 || !in ? 1 : 0)) * kTRows * (2 + D);
-        ml[i] = __ldcg(reinterpret_cast<const float2 *>(part + kTRows * D + 2 * r));
+        const int p = c + i * step;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p > last) continue;
+        const float *part = a.ws + (static_cast<int64_t>(p) * 2 + (p == c0)) * C::kPart;
+        ml[i] = __ldcg(reinterpret_cast<const float2 *>(part + C::kRows * D + 2 * r));
         o[i] = __ldcg(reinterpret_cast<const float4 *>(part + r * D + d));
-        if (!in) ml[i] = make_float2(-INFINITY, 0.f), o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float top = M;
 #pragma unroll
@@ -73,27 +80,49 @@ __device__ __forceinline__ void join_unit(const TreeArgs &a, int b, int h, int r
         O[3] += o[i].w * f;
       }
     }
+    if (to) {
+      __syncthreads();  // a row's (m, l) is read by several threads
+      if (!in_rows) continue;
+      if (d == 0) *reinterpret_cast<float2 *>(to + C::kRows * D + 2 * r) = make_float2(M, dead ? -1.f : L);
+      *reinterpret_cast<float4 *>(to + r * D + d) = make_float4(O[0], O[1], O[2], O[3]);
+    } else if (in_rows) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
-    *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d) =
-        make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
+      for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
+      *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + row / g * a.os[1] + (h * g + row % g) * a.os[2] + d) =
+          make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
+    }
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_attn_kernel(TreeArgs a) {
-  using C = TreeCfg<D>;
-  constexpr int kStages = C::kStages;
+// Counts this CTA in at `count` (its stores before are in memory first). True for the last
+// of `n`, which sees the stores of all of them and leaves the counter at 0.
+__device__ __forceinline__ bool last_of(unsigned *count, int n, bool *flag) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // release: the block's stores (ordered before by the barrier); acquire: the others'
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    *flag = before == static_cast<unsigned>(n - 1);
+    if (*flag) *count = 0;  // ready for the next call
+  }
+  __syncthreads();
+  return *flag;
+}
+
+template <int D, int kM>
+__global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D, kM>::kCtasPerSm) tree_attn_kernel(TreeArgs a) {
+  using C = TreeCfg<D, kM>;
+  constexpr int kStages = C::kStages, kRows = C::kRows;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red_m[kTWarps][kTRows], red_l[kTWarps][kTRows];
+  __shared__ float red_m[kTWarps][kRows], red_l[kTWarps][kRows];
   __shared__ int pref[kTMaxBatch + 1], warp_sums[kTWarps];
   __shared__ TreePaths tree;
-  __shared__ __align__(16) uint32_t paths[kTRows][kTMaxNodes / 32];
+  __shared__ __align__(16) uint32_t paths[kRows][kTMaxNodes / 32];
   __shared__ uint32_t usable[kTMaxNodes / 32];
   __shared__ bool last_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
   Stage<D> *ring = reinterpret_cast<Stage<D> *>(smem) + warp * kStages;
-  float (*red_o)[kTRows][D] = reinterpret_cast<float (*)[kTRows][D]>(smem);
+  float (*red_o)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(smem);
   pdl_launch_dependents();
   pdl_wait();
   cost_prefix<TreeCut, 32 * kTWarps>(a, pref, warp_sums);
@@ -107,7 +136,7 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
 
   for (Segment sg = next_segment<TreeCut>(a, pref, w, w_end); sg.count > 0;
        sg = next_segment<TreeCut>(a, pref, sg.next, w_end)) {
-    const int b = sg.b, h = sg.h, row0 = sg.group * kTRows, first = sg.first, count = sg.count;
+    const int b = sg.b, h = sg.h, row0 = sg.group * kRows, first = sg.first, count = sg.count;
     const int len = cached_len(a, b), ctiles = (len + kTTile - 1) / kTTile;
     const int *table = a.table + static_cast<int64_t>(b) * a.M;
     // the warp's blocks: cached tiles first .. ctiles - 1 (block 4 i + warp of tokens), then nodes
@@ -135,12 +164,16 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) valid[s] = request(s, s);
 
-    WarpAttn<D> at;
-    at.clear();
-    const int r_lo = row0 + gid, r_hi = row0 + gid + 8, rows = a.N * g;
-    const uint16_t *qb = a.q + b * a.qs[0];
-    at.load_q(r_lo < rows ? qb + r_lo / g * a.qs[1] + (h * g + r_lo % g) * a.qs[2] : nullptr,
-              r_hi < rows ? qb + r_hi / g * a.qs[1] + (h * g + r_hi % g) * a.qs[2] : nullptr);
+    WarpAttn<D> at[kM];
+    const int rows = a.N * g;
+    auto q_row = [&](int r) {
+      return r < rows ? a.q + b * a.qs[0] + r / g * a.qs[1] + (h * g + r % g) * a.qs[2] : nullptr;
+    };
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+      at[m].clear();
+      at[m].load_q(q_row(row0 + 16 * m + gid), q_row(row0 + 16 * m + gid + 8));
+    }
     if (first + count > ctiles) {  // the tree's nodes are part of this piece: their paths
       if (warp == 0) {
         tree_paths(tree, a.parents + static_cast<int64_t>(b) * a.N, a.N);
@@ -149,7 +182,7 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
           const unsigned all = __ballot_sync(0xffffffffu, tree.up[k * 32 + lane] == -1);
           if (lane == 0) usable[k] = all;
         }
-        if (lane < kTRows) {
+        if (lane < kRows) {
           const int i = (row0 + lane) / g;
           *reinterpret_cast<uint4 *>(paths[lane]) = i < a.N ? tree.bits[i] : make_uint4(0u, 0u, 0u, 0u);
         }
@@ -167,7 +200,8 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
         valid[(s + kLast) % kStages] = request(i + kLast, (s + kLast) % kStages);
         if (valid[s] > 0) {
           const uint32_t see[2] = {0xffffu >> (16 - valid[s]), 0xffffu >> (16 - valid[s])};
-          at.step(ring[s], a.scale_log2, see);
+#pragma unroll
+          for (int m = 0; m < kM; ++m) at[m].step(ring[s], a.scale_log2, see);
         }
       }
     }
@@ -183,7 +217,9 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
       cp_async_commit();
       cp_async_wait<0>();
       __syncwarp();
-      const uint32_t see[2] = {paths[gid][j0 >> 5] >> (j0 & 31) & 0xffffu, paths[gid + 8][j0 >> 5] >> (j0 & 31) & 0xffffu};
+      uint32_t see[kM][2];
+#pragma unroll
+      for (int m = 0; m < 2 * kM; ++m) see[m >> 1][m & 1] = paths[8 * m + gid][j0 >> 5] >> (j0 & 31) & 0xffffu;
       // a masked token's probability is 0, but 0 * inf is not: values that are not finite
       // leave the tile and are added to the rows that see them
       bool odd = false;
@@ -202,8 +238,11 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
         if (change) *p = y;
         odd |= change;
       }
-      if (__any_sync(0xffffffffu, odd)) {
-        __syncwarp();
+      odd = __any_sync(0xffffffffu, odd);
+      __syncwarp();
+#pragma unroll
+      for (int m = 0; m < kM; ++m) at[m].step(st, a.scale_log2, see[m]);
+      if (odd) {  // after the step, which rescales O
         for (int t = 0; t < 16; ++t) {
           if (!(can >> t & 1u)) continue;
           const uint16_t *vt = a.v_new + at0 + t * a.ks[1];
@@ -213,75 +252,80 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
             for (int e = 0; e < 2; ++e) {
               const float f = bf16_bits_to_float(ld_act_u16(vt + 8 * j + 2 * tid + e));
               if (isfinite(f)) continue;
-              if (see[0] >> t & 1u) at.o[j][e] += f;
-              if (see[1] >> t & 1u) at.o[j][2 + e] += f;
+#pragma unroll
+              for (int m = 0; m < 2 * kM; ++m)
+                if (see[m >> 1][m & 1] >> t & 1u) at[m >> 1].o[j][2 * (m & 1) + e] += f;
             }
         }
       }
-      at.step(st, a.scale_log2, see);
       __syncwarp();  // done with the stage
     }
-    at.finish();
-    __syncthreads();  // every warp is done with the V tiles
-    if (tid == 0) {
-      red_m[warp][gid] = at.m[0];
-      red_m[warp][gid + 8] = at.m[1];
-      red_l[warp][gid] = at.l[0];
-      red_l[warp][gid + 8] = at.l[1];
-    }
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      *reinterpret_cast<float2 *>(&red_o[warp][gid][8 * j + 2 * tid]) = make_float2(at.o[j][0], at.o[j][1]);
-      *reinterpret_cast<float2 *>(&red_o[warp][gid + 8][8 * j + 2 * tid]) = make_float2(at.o[j][2], at.o[j][3]);
+    for (int m = 0; m < kM; ++m) at[m].finish();
+    __syncthreads();  // every warp is done with the V tiles
+#pragma unroll
+    for (int m = 0; m < 2 * kM; ++m) {
+      const WarpAttn<D> &x = at[m >> 1];
+      const int r = 8 * m + gid, e = m & 1;
+      if (tid == 0) {
+        red_m[warp][r] = x.m[e];
+        red_l[warp][r] = x.l[e];
+      }
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2 *>(&red_o[warp][r][8 * j + 2 * tid]) = make_float2(x.o[j][2 * e], x.o[j][2 * e + 1]);
     }
     __syncthreads();
     const bool whole = count == sg.tiles;
     const bool has_tree = first + count > ctiles;
-    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * kTRows * (2 + D);  // O, then (m, l)
-    for (int idx = threadIdx.x; idx < kTRows * D; idx += 32 * kTWarps) {
-      const int r = idx / D, d = idx % D;
-      float M = -INFINITY, L = 0.f, O = 0.f;
+    float *part = a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (first == 0 ? 1 : 0)) * C::kPart;
+#pragma unroll 2
+    for (int idx = threadIdx.x; idx < kRows * D / 4; idx += 32 * kTWarps) {
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4, rr = row0 + r;
+      if (rr >= rows) break;
+      float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < kTWarps; ++q) M = fmaxf(M, red_m[q][r]);
 #pragma unroll
       for (int q = 0; q < kTWarps; ++q) {
         const float f = rescale(red_m[q][r], M);
+        const float4 o = *reinterpret_cast<const float4 *>(&red_o[q][r][d]);
         L += red_l[q][r] * f;
-        O += red_o[q][r][d] * f;
+        O[0] += o.x * f;
+        O[1] += o.y * f;
+        O[2] += o.z * f;
+        O[3] += o.w * f;
       }
       // an unused node: its path is empty (a used one holds the node itself)
       bool dead = false;
       if (has_tree) dead = (paths[r][0] | paths[r][1] | paths[r][2] | paths[r][3]) == 0;
       if (whole) {
-        const int rr = row0 + r;
-        if (rr < rows)
-          a.out[b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d] =
-              float_to_bf16_bits(dead ? 0.f : normalised(O, L));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] = dead ? 0.f : normalised(O[e], L);
+        *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d) =
+            make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
       } else {
-        if (d == 0) {
-          part[kTRows * D + 2 * r] = M;
-          part[kTRows * D + 2 * r + 1] = dead ? -1.f : L;  // -1: the join writes zeros
-        }
-        part[r * D + d] = O;
+        if (d == 0) *reinterpret_cast<float2 *>(part + kRows * D + 2 * r) = make_float2(M, dead ? -1.f : L);  // -1: the join writes zeros
+        *reinterpret_cast<float4 *>(part + r * D + d) = make_float4(O[0], O[1], O[2], O[3]);
       }
     }
-    __syncthreads();  // shared memory is used again
-    if (!whole) {
-      // this piece's part is in memory before it is counted; the one that completes the
-      // count has seen all of them
+    if (whole) {
+      __syncthreads();  // shared memory is used again
+    } else {
       const int unit = h * a.groups + sg.group, cost = sg.tiles + TreeCut::kUnitCost;
       const int64_t start = static_cast<int64_t>(pref[b]) * a.Hkv * a.groups + static_cast<int64_t>(unit) * cost;
       const int c0 = piece_of(total, start + TreeCut::kUnitCost, pieces), c1 = piece_of(total, start + cost - 1, pieces);
-      unsigned *count = a.counts + static_cast<int64_t>(b) * a.Hkv * a.groups + unit;
-      if (threadIdx.x == 0) {
-        // release: the block's stores (ordered before by the barrier); acquire: the others'
-        unsigned before;
-        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
-        last_s = before == static_cast<unsigned>(c1 - c0);
-        if (last_s) *count = 0;  // ready for the next call
+      unsigned *count = a.counts + 2 * gridDim.x + static_cast<int64_t>(b) * a.Hkv * a.groups + unit;
+      if (c1 - c0 < 2 * kJoin) {
+        if (last_of(count, c1 - c0 + 1, &last_s)) join<D, kM>(a, b, h, row0, c0, c0, c1, 1, nullptr);
+      } else {
+        const int p0 = c0 + (static_cast<int>(blockIdx.x) - c0) / kJoin * kJoin, p1 = min(p0 + kJoin - 1, c1);
+        const int place = 2 * p0 + (p0 == c0);  // as the partial's: one unit per place
+        if (last_of(a.counts + place, p1 - p0 + 1, &last_s)) {
+          join<D, kM>(a, b, h, row0, c0, p0, p1, 1, a.ws + static_cast<int64_t>(place) * C::kPart);
+          if (last_of(count, (c1 - c0) / kJoin + 1, &last_s)) join<D, kM>(a, b, h, row0, c0, c0, c1, kJoin, nullptr);
+        }
       }
-      __syncthreads();
-      if (last_s) join_unit<D>(a, b, h, row0, c0, c1);
       __syncthreads();
     }
   }
@@ -291,23 +335,35 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D>::kCtasPerSm) tree_att
 
 using namespace iron;
 
-static int tree_pieces(int head_dim) {
-  return sm_count() * (head_dim == 128 ? TreeCfg<128>::kCtasPerSm : TreeCfg<64>::kCtasPerSm);
+static int tree_pieces(int head_dim, int unit) {
+  return sm_count() * (head_dim == 64 && unit == 16 ? TreeCfg<64, 1>::kCtasPerSm : TreeCfg<64, 2>::kCtasPerSm);
+}
+static_assert(TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 1>::kCtasPerSm && TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 2>::kCtasPerSm);
+
+// Rows of a unit. 32 read K and V half as often as 16; 16 are cut finer and have less to
+// join. 32 are taken where a CTA's share of full tables is at least 32 tiles of 16 rows.
+// B200, 32 rows, us with 16 / 32: head dim 64, 1 x 4608 tokens (3 tiles) 18 / 20, 4 x 4608 (10)
+// 24 / 32, 16 x 4608 (41) 52 / 49, 64 x 2304 (83) 113 / 89; head dim 128, 1 x 16384 (14) 37 / 42,
+// 8 x 32768 (221) 371 / 225.
+static int unit_rows(int B, int rows, int Hkv, int head_dim, int64_t longest) {
+  if (rows <= 16) return 16;
+  const int64_t tiles = static_cast<int64_t>(B) * Hkv * ((rows + 15) / 16) * ((longest + kTTile - 1) / kTTile);
+  return tiles < 32LL * tree_pieces(head_dim, 16) ? 16 : 32;
 }
 
-// Bytes of a counter per unit of the mma.sync form, rounded up to 16.
-static size_t tree_counters(int B, int N, int Hq, int Hkv) {
-  const size_t groups = (static_cast<size_t>(N) * (Hq / Hkv) + kTRows - 1) / kTRows;
-  return (B * Hkv * groups * sizeof(unsigned) + 15) / 16 * 16;
+// Bytes of the mma.sync form's counters, two per piece and one per unit, rounded up to 16.
+static size_t tree_counters(int B, int N, int Hq, int Hkv, int head_dim) {
+  const size_t units = static_cast<size_t>(B) * Hkv * ((static_cast<size_t>(N) * (Hq / Hkv) + 15) / 16);
+  return ((2 * static_cast<size_t>(tree_pieces(head_dim, 16)) + units) * sizeof(unsigned) + 15) / 16 * 16;
 }
 
 extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
   if (batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  // the counters of the units that are cut, then the partials
-  const size_t few = tree_counters(batch, num_nodes, num_heads, kv_heads) +
-                     static_cast<size_t>(tree_pieces(head_dim)) * 2 * kTRows * (2 + head_dim) * sizeof(float);
-  const size_t many = tree_counters(batch, num_nodes, num_heads, kv_heads) + tree_tc_workspace(head_dim);
-  return few > many ? few : many;
+  // the counters, then the partials of any form
+  const size_t f16 = static_cast<size_t>(tree_pieces(head_dim, 16)) * 2 * 16 * (2 + head_dim) * sizeof(float);
+  const size_t f32 = static_cast<size_t>(tree_pieces(head_dim, 32)) * 2 * 32 * (2 + head_dim) * sizeof(float);
+  const size_t few = f16 > f32 ? f16 : f32, many = tree_tc_workspace(head_dim);
+  return tree_counters(batch, num_nodes, num_heads, kv_heads, head_dim) + (few > many ? few : many);
 }
 
 // Rows of a (sequence, kv head) from which the tensor cores' 128-row tiles are used.
@@ -321,6 +377,17 @@ static bool use_tensor_form(const TreeArgs &a) {
     if (n > 1 && (a.ks[i] <= 0 || a.ks[i] >= (1LL << 38))) return false;
   }
   return a.N * (a.Hq / a.Hkv) >= kTensorRows && a.scale_log2 >= 1e-30f;
+}
+
+template <int D, int kM>
+static int launch_few(const TreeArgs &a, cudaStream_t s) {
+  using C = TreeCfg<D, kM>;
+  static PerDeviceOnce once;
+  const int st = once.run([] {
+    return call_status(cudaFuncSetAttribute(tree_attn_kernel<D, kM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  });
+  if (st != IRON_OK) return st;
+  return launch(tree_attn_kernel<D, kM>, dim3(tree_pieces(D, C::kRows)), dim3(32 * kTWarps), C::kSmem, s, true, a);
 }
 
 extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
@@ -352,7 +419,8 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.parents = parents;
   a.out = out;
   a.counts = static_cast<unsigned *>(workspace);
-  a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + tree_counters(c->slots, num_nodes, num_heads, c->kv_heads));
+  a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) +
+                                   tree_counters(c->slots, num_nodes, num_heads, c->kv_heads, c->head_dim));
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i];
     a.ks[i] = kv_strides[i];
@@ -362,23 +430,15 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.N = num_nodes;
   a.Hq = num_heads;
   a.Hkv = c->kv_heads;
-  a.groups = (num_nodes * g + kTRows - 1) / kTRows;
+  const int unit = unit_rows(c->slots, num_nodes * g, c->kv_heads, c->head_dim, static_cast<int64_t>(c->max_pages) * c->page_size);
+  a.groups = (num_nodes * g + unit - 1) / unit;
   a.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   a.M = c->max_pages;
   a.P = c->num_pages;
   a.scale_log2 = scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = c->head_dim == 128;
   if (use_tensor_form(a)) return tree_tc_launch(a, c->head_dim, s);
-  const int pieces = tree_pieces(c->head_dim);
-  static PerDeviceOnce once;
-  int st = once.run([] {
-    cudaError_t e = cudaFuncSetAttribute(tree_attn_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeCfg<64>::kSmem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(tree_attn_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeCfg<128>::kSmem);
-    return call_status(e);
-  });
-  if (st != IRON_OK) return st;
-  return launch(wide ? tree_attn_kernel<128> : tree_attn_kernel<64>, dim3(pieces), dim3(32 * kTWarps),
-                wide ? TreeCfg<128>::kSmem : TreeCfg<64>::kSmem, s, true, a);
+  const bool two = unit == 32;
+  if (c->head_dim == 128) return two ? launch_few<128, 2>(a, s) : launch_few<128, 1>(a, s);
+  return two ? launch_few<64, 2>(a, s) : launch_few<64, 1>(a, s);
 }

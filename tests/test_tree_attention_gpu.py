@@ -107,6 +107,41 @@ def test_many_tiles_per_piece(N, D):
     run([4096, 2999, 2049, 100, 3100, 0, 4000, 640], N, 32, 8, D, 64, seed=N)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [5, 8])
+def test_few_rows_and_tables_for_long_sequences(N, D):
+    """17 to 32 rows per kv head where full tables would be a lot of work."""
+    lens = [0, 1, 700, 2048, 64, 5000, 130, 63, 1025, 16, 400, 129, 2999, 15, 65, 300]
+    for kind in ("random", "ragged"):
+        run(lens, N, 32, 8, D, 64, kind=kind, seed=N, width=300)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_units_in_many_pieces(D):
+    run([40001], 2, 1, 1, D, 64, seed=1)
+    run([20003, 300], 4, 16, 4, D, 64, seed=2)
+    run([30011], 8, 8, 2, D, 64, kind="ragged", seed=3)
+
+
+@pytest.mark.parametrize("Hq,width", [(8, 16), (32, 16), (32, 1000), (64, 16)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinite_values_reach_the_rows_that_see_them(Hq, width, D):
+    cache = Cache([70, 0, 900, 130], 8, D, 64, 5, width=width)
+    g = gen(5)
+    q, kn, vn = randn(g, 4, 8, Hq, D), randn(g, 4, 8, 8, D), randn(g, 4, 8, 8, D)
+    parents = [[-1, 0, 1, 0, 3, -1, 5, 2]] * 4
+    vn[:, 3, :, 7] = math.inf
+    vn[:, 6, :, 9] = -math.inf
+    out = torch.full_like(q, math.nan)
+    operator(cache, 4, 8, Hq).get_callable()(q, kn, vn, cache.k, cache.v, cache.table, cache.lens,
+                                             torch.tensor(parents, dtype=torch.int32, device="cuda"), out)
+    for n in range(8):
+        x = out[:, n].double()
+        assert bool((x[..., 7] == math.inf).all()) == (n in (3, 4)) and bool((x[..., 9] == -math.inf).all()) == (n == 6)
+        x[..., 7] = x[..., 9] = 0
+        assert bool(torch.isfinite(x).all())
+
+
 def test_batch_of_many():
     rng = random.Random(2)
     run([rng.randint(0, 200) for _ in range(300)], 2, 4, 1, 64, 32, seed=2)
