@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(32 * kTWarps, TreeCfg<D, kM>::kCtasPerSm) tree
         *reinterpret_cast<uint2 *>(a.out + b * a.os[0] + rr / g * a.os[1] + (h * g + rr % g) * a.os[2] + d) =
             make_uint2(pack_bf16x2(O[0], O[1]), pack_bf16x2(O[2], O[3]));
       } else {
-        if (d == 0) *reinterpret_cast<float2 *>(part + kRows * D + 2 * r) = make_float2(M, dead ? -1.f : L);  // -1: the join writes zeros
+        // a sum of -1: the join writes zeros
+        if (d == 0) *reinterpret_cast<float2 *>(part + kRows * D + 2 * r) = make_float2(M, dead ? -1.f : L);
         *reinterpret_cast<float4 *>(part + r * D + d) = make_float4(O[0], O[1], O[2], O[3]);
       }
     }
@@ -338,17 +339,21 @@ using namespace iron;
 static int tree_pieces(int head_dim, int unit) {
   return sm_count() * (head_dim == 64 && unit == 16 ? TreeCfg<64, 1>::kCtasPerSm : TreeCfg<64, 2>::kCtasPerSm);
 }
-static_assert(TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 1>::kCtasPerSm && TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 2>::kCtasPerSm);
+static_assert(TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 1>::kCtasPerSm);
+static_assert(TreeCfg<64, 2>::kCtasPerSm == TreeCfg<128, 2>::kCtasPerSm);
 
 // Rows of a unit. 32 read K and V half as often as 16; 16 are cut finer and have less to
 // join. 32 are taken where a CTA's share of full tables is at least 32 tiles of 16 rows.
 // B200, 32 rows, us with 16 / 32: head dim 64, 1 x 4608 tokens (3 tiles) 18 / 20, 4 x 4608 (10)
 // 24 / 32, 16 x 4608 (41) 52 / 49, 64 x 2304 (83) 113 / 89; head dim 128, 1 x 16384 (14) 37 / 42,
 // 8 x 32768 (221) 371 / 225.
-static int unit_rows(int B, int rows, int Hkv, int head_dim, int64_t longest) {
-  if (rows <= 16) return 16;
-  const int64_t tiles = static_cast<int64_t>(B) * Hkv * ((rows + 15) / 16) * ((longest + kTTile - 1) / kTTile);
-  return tiles < 32LL * tree_pieces(head_dim, 16) ? 16 : 32;
+static int unit_rows(int rows, int64_t tiles, int head_dim) {
+  return rows > 16 && tiles >= 32LL * tree_pieces(head_dim, 16) ? 32 : 16;
+}
+// 64-token tiles of 16 rows that full tables hold.
+static int64_t full_tiles(const iron_page_pool *c, int rows) {
+  const int64_t longest = static_cast<int64_t>(c->max_pages) * c->page_size;
+  return static_cast<int64_t>(c->slots) * c->kv_heads * ((rows + 15) / 16) * ((longest + kTTile - 1) / kTTile);
 }
 
 // Bytes of the mma.sync form's counters, two per piece and one per unit, rounded up to 16.
@@ -366,17 +371,25 @@ extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int n
   return tree_counters(batch, num_nodes, num_heads, kv_heads, head_dim) + (few > many ? few : many);
 }
 
-// Rows of a (sequence, kv head) from which the tensor cores' 128-row tiles are used.
-constexpr int kTensorRows = 33;
+// The tensor cores' 128-row tiles are used from kTensorRows rows of a (sequence, kv head) on,
+// where the form above would need a second unit of 32; but up to kFewRows rows only if full
+// tables hold more than kFewTiles tiles of 16 rows: that form's pipeline takes about 13 us
+// (head dim 64) or 18 (128) to fill and drain. B200, us, here / there: 32 rows, 16 x 4608 tokens
+// at head dim 64 49 / 60, 8 x 32768 at 128 231 / 296; 36 rows 74 / 60 and 422 / 296; 64 rows,
+// 1 x 300 (160 tiles) 9.9 / 13.5, 1 x 4608 (2304) 21 / 22 and at 128 30 / 40, 4 x 4608 (9216)
+// 32 / 27 and 55 / 41; 104 rows, 1 x 2304 (2016) 19 / 20 and 28 / 36; 256 rows, 1 x 300 at 128
+// (640) 26 / 21.
+constexpr int kTensorRows = 33, kFewRows = 128, kFewTiles = 2560;
 
 // The tcgen05 form takes positive scales that do not vanish in log2 units, and new rows
 // whose strides TMA takes (not 0: broadcast views go to the other form).
-static bool use_tensor_form(const TreeArgs &a) {
+static bool use_tensor_form(const TreeArgs &a, int64_t tiles) {
   for (int i = 0; i < 3; ++i) {
     const int n = i == 0 ? a.B : i == 1 ? a.N : a.Hkv;
     if (n > 1 && (a.ks[i] <= 0 || a.ks[i] >= (1LL << 38))) return false;
   }
-  return a.N * (a.Hq / a.Hkv) >= kTensorRows && a.scale_log2 >= 1e-30f;
+  const int rows = a.N * (a.Hq / a.Hkv);
+  return rows >= kTensorRows && (rows > kFewRows || tiles > kFewTiles) && a.scale_log2 >= 1e-30f;
 }
 
 template <int D, int kM>
@@ -430,14 +443,15 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.N = num_nodes;
   a.Hq = num_heads;
   a.Hkv = c->kv_heads;
-  const int unit = unit_rows(c->slots, num_nodes * g, c->kv_heads, c->head_dim, static_cast<int64_t>(c->max_pages) * c->page_size);
+  const int64_t tiles = full_tiles(c, num_nodes * g);
+  const int unit = unit_rows(num_nodes * g, tiles, c->head_dim);
   a.groups = (num_nodes * g + unit - 1) / unit;
   a.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   a.M = c->max_pages;
   a.P = c->num_pages;
   a.scale_log2 = scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (use_tensor_form(a)) return tree_tc_launch(a, c->head_dim, s);
+  if (use_tensor_form(a, tiles)) return tree_tc_launch(a, c->head_dim, s);
   const bool two = unit == 32;
   if (c->head_dim == 128) return two ? launch_few<128, 2>(a, s) : launch_few<128, 1>(a, s);
   return two ? launch_few<64, 2>(a, s) : launch_few<64, 1>(a, s);

@@ -8,17 +8,25 @@
 // stream 0 then joins both results, whose rows lie in the same TMEM lanes.
 //
 // Warps: 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns one row: no shuffles), 8
-// issues the MMAs, 9 loads (TMA, one box per page and 64 columns).
-//   S = Q K^T     128 x 128 x D, both operands in shared memory (K-major)
-//   P -> TMEM     over S: bf16 hi and lo parts, 64 columns each (P = hi + lo to 2^-16: one
-//                 bf16 would double the error of the rounded output)
-//   O += P V      128 x D x 128, twice; A from TMEM, V as it lies in the page (MN-major)
-// TMEM: S0, S1 128 columns each, O0, O1 D each. O is rescaled only when a row's maximum
-// has grown by more than 2^8 (P stays below 2^8, exact in the sums' fp32 range).
+// and 9 issue the MMAs of stream 0 and 1, 10 loads (TMA, one box per page and 64 columns),
+// 11 finds the nodes' paths and zeroes the rows of V that hold nothing.
+//   S = Q K^T     128 x 128 x D (D = 128: x 64), both operands in shared memory (K-major)
+//   P -> TMEM     64 tokens at a time, in columns of its own: bf16 hi and lo parts (P = hi +
+//                 lo to 2^-16: one bf16 would double the error of the rounded output)
+//   O += P V      128 x D x 64, hi then lo; A from TMEM, V as it lies in the page (MN-major)
+// S is read into registers whole, so the MMAs of the next S run under this one's softmax.
+// TMEM (512 columns): S0, S1, O0, O1, P0, P1. O is rescaled only when a row's maximum has
+// grown by more than 2^8 (P stays below 2^8, exact in the sums' fp32 range).
 //
-// Bounds: D = 128: per tile and stream 512 cycles of S and 1024 of P V against 1024 of ex2
-// (16 per cycle and SM), so the tensor cores; D = 64: ex2. What a tile must not hold (past
-// the length, unused nodes) is masked in S and zeroed in V.
+// Bounds (B200): per 128 tokens and stream 1024 cycles of ex2 (16 per cycle and SM for 128
+// rows), and on the tensor cores 250 of S and 530 of P V at D = 64, 770 and 960 at D = 128
+// (measured alone: S of 64 columns 48 cycles per MMA, of 128 columns 62; P V 33 and 60).
+// 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 107 us, D = 128 120; without the
+// MMAs 100, without ex2 88, without all arithmetic of the softmax 71 (D = 64): no unit is
+// full, and the chain from S through TMEM and registers to P sets the pace. 8 sequences of
+// 32768 tokens, D = 128: 282 us, tensor cores 70 % busy (335 in long runs, at the power
+// limit). What a tile must not hold (past the length, unused nodes) is masked in S and
+// zeroed in V.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -214,231 +222,231 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 10) {
-    // ---- loads ----
-    if (lane == 0) {
-      tc::prefetch_tmap(&maps.k);
-      tc::prefetch_tmap(&maps.v);
-    }
-    const int page = 1 << a.page_shift, ppt = kTile >> a.page_shift;  // pages per tile
-    bool ok = true;
-    int it = 0;
-    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
-         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
-      const int len = cached_len(a, sg.b), ctiles = (len + kTile - 1) / kTile;
-      const int *table = a.table + static_cast<int64_t>(sg.b) * a.M;
-      // 32 table entries at a time, the next ones requested while these are used
-      const int per = 32 >> (7 - a.page_shift);  // tiles per 32 entries
-      auto entries = [&](int tile) {
-        const int e = tile * ppt + lane;
-        return e < a.M ? ld_act_i32(table + e) : -1;
-      };
-      int cur = entries(sg.first), next = entries(sg.first + per), used = 0;
-      for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
-        const int s = it % S;
-        const bool tree = i >= ctiles;
-        // this tile's pages: lane l < ppt holds page l and its valid rows
-        if (used == per) {
-          cur = next;
-          next = entries(i + per);
-          used = 0;
+      // ---- loads ----
+      if (lane == 0) {
+        tc::prefetch_tmap(&maps.k);
+        tc::prefetch_tmap(&maps.v);
+      }
+      const int page = 1 << a.page_shift, ppt = kTile >> a.page_shift;  // pages per tile
+      bool ok = true;
+      int it = 0;
+      for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+           sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
+        const int len = cached_len(a, sg.b), ctiles = (len + kTile - 1) / kTile;
+        const int *table = a.table + static_cast<int64_t>(sg.b) * a.M;
+        // 32 table entries at a time, the next ones requested while these are used
+        const int per = 32 >> (7 - a.page_shift);  // tiles per 32 entries
+        auto entries = [&](int tile) {
+          const int e = tile * ppt + lane;
+          return e < a.M ? ld_act_i32(table + e) : -1;
+        };
+        int cur = entries(sg.first), next = entries(sg.first + per), used = 0;
+        for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
+          const int s = it % S;
+          const bool tree = i >= ctiles;
+          // this tile's pages: lane l < ppt holds page l and its valid rows
+          if (used == per) {
+            cur = next;
+            next = entries(i + per);
+            used = 0;
+          }
+          const int pid = __shfl_sync(0xffffffffu, cur, (used * ppt + lane) & 31);
+          ++used;
+          int n = 0;
+          if (!tree && lane < ppt && pid >= 0 && pid < a.P) n = max(0, min(page, len - i * kTile - lane * page));
+          uint32_t bits = 0;  // lane w < 4: the valid tokens of word w
+          for (int p = 0; p < ppt; ++p) {
+            const int np = __shfl_sync(0xffffffffu, n, p);
+            const int lo = max(p * page, 32 * lane), hi = min(p * page + np, 32 * lane + 32);
+            if (hi > lo) bits |= (hi - lo == 32 ? 0xffffffffu : (1u << (hi - lo)) - 1u) << (lo & 31);
+          }
+          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, n > 0));
+          const uint32_t bytes = tree ? C::kOperand : boxes * page * D * 2;
+          const uint32_t parity = ((it / S) & 1) ^ 1;
+          ok = __all_sync(0xffffffffu, wait_phase(bars.kempty<S>(s), parity));
+          if (!ok) break;
+          if (lane < 4) masks[it % kMasks][lane] = bits;
+          __syncwarp();
+          if (lane == 0) {
+            tc::arrive(bars.mask<S>(it % kMasks));
+            tc::expect_tx(bars.kfull<S>(s), bytes);
+          }
+          __syncwarp();
+          auto load = [&](const CUtensorMap *pages, const CUtensorMap *fresh, uint32_t dst, uint32_t bar) {
+            if (tree) {
+              if (lane < C::kPanels) tc::tma_load_4d(dst + lane * C::kPanel, fresh, lane * 64, 0, sg.h, sg.b, bar);
+            } else if (n > 0) {
+#pragma unroll
+              for (int c = 0; c < C::kPanels; ++c)
+                tc::tma_load_4d(dst + c * C::kPanel + lane * page * 128, pages, c * 64, 0, sg.h, pid, bar);
+            }
+          };
+          load(&maps.k, &maps.k_new, k0 + s * C::kOperand, bars.kfull<S>(s));
+          ok = __all_sync(0xffffffffu, wait_phase(bars.vempty<S>(s), parity));
+          if (!ok) {
+            // this tile's K is on its way already: let it land
+            wait_phase(bars.kfull<S>(s), (it / S) & 1);
+            break;
+          }
+          if (lane == 0) tc::expect_tx(bars.vfull<S>(s), bytes);
+          __syncwarp();
+          load(&maps.v, &maps.v_new, v0 + s * C::kOperand, bars.vfull<S>(s));
         }
-        const int pid = __shfl_sync(0xffffffffu, cur, (used * ppt + lane) & 31);
-        ++used;
-        int n = 0;
-        if (!tree && lane < ppt && pid >= 0 && pid < a.P) n = max(0, min(page, len - i * kTile - lane * page));
-        uint32_t bits = 0;  // lane w < 4: the valid tokens of word w
-        for (int p = 0; p < ppt; ++p) {
-          const int np = __shfl_sync(0xffffffffu, n, p);
-          const int lo = max(p * page, 32 * lane), hi = min(p * page + np, 32 * lane + 32);
-          if (hi > lo) bits |= (hi - lo == 32 ? 0xffffffffu : (1u << (hi - lo)) - 1u) << (lo & 31);
+      }
+      if (!ok) {
+        if (lane == 0) atomicCAS(&g_tree_status, 0u, 1u);
+        // copies in flight land before the CTA's shared memory goes away
+        for (int j = max(0, it - S); j < it; ++j) {
+          wait_phase(bars.kfull<S>(j % S), (j / S) & 1);
+          wait_phase(bars.vfull<S>(j % S), (j / S) & 1);
         }
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, n > 0));
-        const uint32_t bytes = tree ? C::kOperand : boxes * page * D * 2;
-        const uint32_t parity = ((it / S) & 1) ^ 1;
-        ok = __all_sync(0xffffffffu, wait_phase(bars.kempty<S>(s), parity));
-        if (!ok) break;
-        if (lane < 4) masks[it % kMasks][lane] = bits;
-        __syncwarp();
-        if (lane == 0) {
-          tc::arrive(bars.mask<S>(it % kMasks));
-          tc::expect_tx(bars.kfull<S>(s), bytes);
-        }
-        __syncwarp();
-        auto load = [&](const CUtensorMap *pages, const CUtensorMap *fresh, uint32_t dst, uint32_t bar) {
-          if (tree) {
-            if (lane < C::kPanels) tc::tma_load_4d(dst + lane * C::kPanel, fresh, lane * 64, 0, sg.h, sg.b, bar);
-          } else if (n > 0) {
+      }
+    } else if (warp < 10) {
+      // ---- MMAs of stream `s`: the warp stays converged, an elected lane issues. (One warp for
+      // both streams was what bound the kernel: its instructions share their scheduler with
+      // two softmax warps, and each stream waited for the other one's turn.) ----
+      const int s = warp - 8;
+      constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, C::kScores);
+      constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
+      bool ok = true;
+      int it0 = 0;
+      uint32_t pc = 0, qc = 0, sn = 0;
+      for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); uniform(sg.count) > 0;
+           sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
+        const Streams st = streams_of(a, sg);
+        const int len = uniform(cached_len(a, sg.b)), ctiles = (len + kTile - 1) / kTile;
+        const int first = uniform(sg.first), n = uniform(st.n[s]);
+        const bool both = uniform(st.both);
+        const int it0s = it0 + (both ? 0 : s), step = both ? 1 : 2;
+        // K and V are released by both streams; a tile that one stream has alone, by it twice
+        const bool twice = !both;
+        auto halves = [&](int j) { return halves_of(a, first + (both ? j : 2 * j + s), ctiles, len); };
+        // S of tile j: all of it (h = 0), or its half h
+        auto scores = [&](int j, int h, bool last) {
+          const int it = it0s + j * step, slot = it % S;
+          ok &= wait_phase(bars.kfull<S>(slot), (it / S) & 1);
+          if (sn > 0) ok &= wait_phase(bars.sfree<S>(s), (sn - 1) & 1);
+          ++sn;
+          tc::fence_after_sync();
+          // a step of the start address is a step of the descriptor's low bits (16-byte units)
+          const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
+          const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand + h * (C::kPanel / 2));
+          if (tc::elect_one()) {
 #pragma unroll
             for (int c = 0; c < C::kPanels; ++c)
-              tc::tma_load_4d(dst + c * C::kPanel + lane * page * 128, pages, c * 64, 0, sg.h, pid, bar);
-          }
-        };
-        load(&maps.k, &maps.k_new, k0 + s * C::kOperand, bars.kfull<S>(s));
-        ok = __all_sync(0xffffffffu, wait_phase(bars.vempty<S>(s), parity));
-        if (!ok) {
-          // this tile's K is on its way already: let it land
-          wait_phase(bars.kfull<S>(s), (it / S) & 1);
-          break;
-        }
-        if (lane == 0) tc::expect_tx(bars.vfull<S>(s), bytes);
-        __syncwarp();
-        load(&maps.v, &maps.v_new, v0 + s * C::kOperand, bars.vfull<S>(s));
-      }
-    }
-    if (!ok) {
-      if (lane == 0) atomicCAS(&g_tree_status, 0u, 1u);
-      // copies in flight land before the CTA's shared memory goes away
-      for (int j = max(0, it - S); j < it; ++j) {
-        wait_phase(bars.kfull<S>(j % S), (j / S) & 1);
-        wait_phase(bars.vfull<S>(j % S), (j / S) & 1);
-      }
-    }
-    } else if (warp < 10) {
-    // ---- MMAs of stream `s`: the warp stays converged, an elected lane issues. (One warp for
-    // both streams was what bound the kernel: its instructions share their scheduler with
-    // two softmax warps, and each stream waited for the other one's turn.) ----
-    const int s = warp - 8;
-    constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, C::kScores);
-    constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
-    bool ok = true;
-    int it0 = 0;
-    uint32_t pc = 0, qc = 0, sn = 0;
-    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); uniform(sg.count) > 0;
-         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
-      const Streams st = streams_of(a, sg);
-      const int len = uniform(cached_len(a, sg.b)), ctiles = (len + kTile - 1) / kTile;
-      const int first = uniform(sg.first), n = uniform(st.n[s]);
-      const bool both = uniform(st.both);
-      const int it0s = it0 + (both ? 0 : s), step = both ? 1 : 2;
-      // K and V are released by both streams; a tile that one stream has alone, by it twice
-      const bool twice = !both;
-      auto halves = [&](int j) { return halves_of(a, first + (both ? j : 2 * j + s), ctiles, len); };
-      // S of tile j: all of it (h = 0), or its half h
-      auto scores = [&](int j, int h, bool last) {
-        const int it = it0s + j * step, slot = it % S;
-        ok &= wait_phase(bars.kfull<S>(slot), (it / S) & 1);
-        if (sn > 0) ok &= wait_phase(bars.sfree<S>(s), (sn - 1) & 1);
-        ++sn;
-        tc::fence_after_sync();
-        // a step of the start address is a step of the descriptor's low bits (16-byte units)
-        const uint64_t q = tc::sdesc_kmajor_sw128(q0 + s * C::kOperand);
-        const uint64_t k = tc::sdesc_kmajor_sw128(k0 + slot * C::kOperand + h * (C::kPanel / 2));
-        if (tc::elect_one()) {
 #pragma unroll
-          for (int c = 0; c < C::kPanels; ++c)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::mma_bf16(tmem + C::kTmemS + s * C::kScores, q + c * (C::kPanel >> 4) + kk * 2,
-                           k + c * (C::kPanel >> 4) + kk * 2, idesc_s, c > 0 || kk > 0);
-          tc::mma_commit(bars.sfull<S>(s));
-          if (last) {
-            tc::mma_commit(bars.kempty<S>(slot));
-            if (twice) tc::mma_commit(bars.kempty<S>(slot));
-          }
-        }
-        __syncwarp();
-      };
-      auto values = [&](int j, int h, bool last) {
-        const int it = it0s + j * step, slot = it % S;
-        ok &= wait_phase(bars.vready<S>(slot), (it / S) & 1);
-        ok &= wait_phase(bars.pfull<S>(s), pc++ & 1);
-        tc::fence_after_sync();
-        const uint32_t p = tmem + C::kTmemP + s * 64, o = tmem + C::kTmemO + s * D;
-        const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand + h * (C::kPanel / 2), C::kPanel);
-        if (tc::elect_one()) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::mma_bf16_ts(o, p + part * 32 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || h > 0 || part > 0 || kk > 0);
-          tc::mma_commit(bars.pvdone<S>(s));
-          if (last) {
-            tc::mma_commit(bars.vempty<S>(slot));
-            if (twice) tc::mma_commit(bars.vempty<S>(slot));
-          }
-        }
-        __syncwarp();
-      };
-      if (n > 0) {
-        ok &= wait_phase(bars.qfull<S>(s), qc++ & 1);
-        int k = halves(0);
-        scores(0, 0, C::kScores == kTile || k == 1);
-        // the S that follows goes out before the P V of the last half that the present S
-        // holds: it runs while that half's softmax does, and the softmax never waits for it
-        for (int j = 0; j < n; ++j) {
-          const int next = j + 1 < n ? halves(j + 1) : 0;
-          for (int h = 0; h < k; ++h) {
-            if (C::kScores < kTile && h + 1 < k) scores(j, h + 1, h + 2 == k);
-            else if (h + 1 == k && next > 0) scores(j + 1, 0, C::kScores == kTile || next == 1);
-            values(j, h, h + 1 == k);
-          }
-          k = next;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-      }
-      if (!ok) break;
-      it0 += uniform(sg.count);
-    }
-    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
-    // every MMA issued is done before TMEM is freed
-    if (tc::elect_one()) tc::mma_commit(bars.drain<S>(s));
-    __syncwarp();
-    wait_phase(bars.drain<S>(s), 0);
-    __syncwarp();
-    } else {
-    // ---- preparation: warp 11 ----
-    bool ok = true;
-    int it = 0, trees_done = 0;
-    for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
-         sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
-      const int ctiles = (cached_len(a, sg.b) + kTile - 1) / kTile;
-      TreePaths &tree = trees[trees_done % C::kTrees];
-      if (sg.first + sg.count > ctiles) {
-        tree_paths(tree, a.parents + static_cast<int64_t>(sg.b) * a.N, a.N);
-        tc::arrive_if(lane == 0, bars.paths<S>(trees_done % C::kTrees));
-        ++trees_done;
-      }
-      for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
-        const int slot = it % S;
-        ok = __all_sync(0xffffffffu, wait_phase(bars.vfull<S>(slot), (it / S) & 1));
-        if (!ok) break;
-        const bool nodes = i >= ctiles;
-        const uint4 valid = *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
-        if (nodes || (valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {
-          // rows of V that hold nothing are zeroed, and so are a node's values that are not
-          // finite (0 * inf is not 0; rows that see them get them added at the end)
-          bool odd = false;
-#pragma unroll 1
-          for (int r = lane; r < kTile; r += 32) {
-            const bool keep = nodes ? tree.up[r] == -1 : masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
-            if (keep && !nodes) continue;
-            uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              // lanes start at different pieces of their rows: no bank conflicts
-              uint4 *e = reinterpret_cast<uint4 *>(vrow + (c >> 3) * C::kPanel + (((c & 7) ^ (r & 7)) << 4));
-              uint4 y = keep ? *e : make_uint4(0, 0, 0, 0);
-              bool change = !keep;
-              if (keep) {
-                uint32_t *u = reinterpret_cast<uint32_t *>(&y);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u, change = odd = true;
-                  if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu, change = odd = true;
-                }
-              }
-              if (change) *e = y;
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_bf16(tmem + C::kTmemS + s * C::kScores, q + c * (C::kPanel >> 4) + kk * 2,
+                             k + c * (C::kPanel >> 4) + kk * 2, idesc_s, c > 0 || kk > 0);
+            tc::mma_commit(bars.sfull<S>(s));
+            if (last) {
+              tc::mma_commit(bars.kempty<S>(slot));
+              if (twice) tc::mma_commit(bars.kempty<S>(slot));
             }
           }
-          if (odd) atomicExch(&odd_flag, 1);
-          tc::fence_proxy_async_smem();
+          __syncwarp();
+        };
+        auto values = [&](int j, int h, bool last) {
+          const int it = it0s + j * step, slot = it % S;
+          ok &= wait_phase(bars.vready<S>(slot), (it / S) & 1);
+          ok &= wait_phase(bars.pfull<S>(s), pc++ & 1);
+          tc::fence_after_sync();
+          const uint32_t p = tmem + C::kTmemP + s * 64, o = tmem + C::kTmemO + s * D;
+          const uint64_t v = tc::sdesc_mnmajor_sw128(v0 + slot * C::kOperand + h * (C::kPanel / 2), C::kPanel);
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_bf16_ts(o, p + part * 32 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || h > 0 || part > 0 || kk > 0);
+            tc::mma_commit(bars.pvdone<S>(s));
+            if (last) {
+              tc::mma_commit(bars.vempty<S>(slot));
+              if (twice) tc::mma_commit(bars.vempty<S>(slot));
+            }
+          }
+          __syncwarp();
+        };
+        if (n > 0) {
+          ok &= wait_phase(bars.qfull<S>(s), qc++ & 1);
+          int k = halves(0);
+          scores(0, 0, C::kScores == kTile || k == 1);
+          // the S that follows goes out before the P V of the last half that the present S
+          // holds: it runs while that half's softmax does, and the softmax never waits for it
+          for (int j = 0; j < n; ++j) {
+            const int next = j + 1 < n ? halves(j + 1) : 0;
+            for (int h = 0; h < k; ++h) {
+              if (C::kScores < kTile && h + 1 < k) scores(j, h + 1, h + 2 == k);
+              else if (h + 1 == k && next > 0) scores(j + 1, 0, C::kScores == kTile || next == 1);
+              values(j, h, h + 1 == k);
+            }
+            k = next;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
         }
-        __syncwarp();
-        tc::arrive_if(lane == 0, bars.vready<S>(slot));
+        if (!ok) break;
+        it0 += uniform(sg.count);
       }
-    }
-    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 5u);
+      if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
+      // every MMA issued is done before TMEM is freed
+      if (tc::elect_one()) tc::mma_commit(bars.drain<S>(s));
+      __syncwarp();
+      wait_phase(bars.drain<S>(s), 0);
+      __syncwarp();
+    } else {
+      // ---- preparation: warp 11 ----
+      bool ok = true;
+      int it = 0, trees_done = 0;
+      for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
+           sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
+        const int ctiles = (cached_len(a, sg.b) + kTile - 1) / kTile;
+        TreePaths &tree = trees[trees_done % C::kTrees];
+        if (sg.first + sg.count > ctiles) {
+          tree_paths(tree, a.parents + static_cast<int64_t>(sg.b) * a.N, a.N);
+          tc::arrive_if(lane == 0, bars.paths<S>(trees_done % C::kTrees));
+          ++trees_done;
+        }
+        for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
+          const int slot = it % S;
+          ok = __all_sync(0xffffffffu, wait_phase(bars.vfull<S>(slot), (it / S) & 1));
+          if (!ok) break;
+          const bool nodes = i >= ctiles;
+          const uint4 valid = *reinterpret_cast<const uint4 *>(masks[it % kMasks]);
+          if (nodes || (valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {
+            // rows of V that hold nothing are zeroed, and so are a node's values that are not
+            // finite (0 * inf is not 0; rows that see them get them added at the end)
+            bool odd = false;
+#pragma unroll 1
+            for (int r = lane; r < kTile; r += 32) {
+              const bool keep = nodes ? tree.up[r] == -1 : masks[it % kMasks][r >> 5] >> (r & 31) & 1u;
+              if (keep && !nodes) continue;
+              uint8_t *vrow = smem + 2 * C::kOperand + (S + slot) * C::kOperand + r * 128;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) {
+                // lanes start at different pieces of their rows: no bank conflicts
+                uint4 *e = reinterpret_cast<uint4 *>(vrow + (c >> 3) * C::kPanel + (((c & 7) ^ (r & 7)) << 4));
+                uint4 y = keep ? *e : make_uint4(0, 0, 0, 0);
+                bool change = !keep;
+                if (keep) {
+                  uint32_t *u = reinterpret_cast<uint32_t *>(&y);
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) {
+                    if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u, change = odd = true;
+                    if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu, change = odd = true;
+                  }
+                }
+                if (change) *e = y;
+              }
+            }
+            if (odd) atomicExch(&odd_flag, 1);
+            tc::fence_proxy_async_smem();
+          }
+          __syncwarp();
+          tc::arrive_if(lane == 0, bars.vready<S>(slot));
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 5u);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));

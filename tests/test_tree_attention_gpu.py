@@ -123,7 +123,7 @@ def test_few_units_in_many_pieces(D):
     run([30011], 8, 8, 2, D, 64, kind="ragged", seed=3)
 
 
-@pytest.mark.parametrize("Hq,width", [(8, 16), (32, 16), (32, 1000), (64, 16)])
+@pytest.mark.parametrize("Hq,width", [(8, 16), (32, 16), (32, 1000), (64, 16), (64, 1000)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_infinite_values_reach_the_rows_that_see_them(Hq, width, D):
     cache = Cache([70, 0, 900, 130], 8, D, 64, 5, width=width)
@@ -140,6 +140,39 @@ def test_infinite_values_reach_the_rows_that_see_them(Hq, width, D):
         assert bool((x[..., 7] == math.inf).all()) == (n in (3, 4)) and bool((x[..., 9] == -math.inf).all()) == (n == 6)
         x[..., 7] = x[..., 9] = 0
         assert bool(torch.isfinite(x).all())
+
+
+# The form for many rows is taken up to 128 rows where tables are wide: the cases above again.
+WIDE = 3000
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [9, 20, 32])
+def test_edge_lengths_with_wide_tables(D, N):
+    run(EDGES, N, 8, 2, D, 64, seed=N, width=WIDE)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [64, 128])
+def test_page_sizes_with_wide_tables(page, D):
+    run([1, 300, page, 3 * page + 1, 777], 11, 8, 2, D, page, seed=page, width=4 * WIDE)
+
+
+@pytest.mark.parametrize("N", [9, 15, 16, 17, 31, 32])
+def test_node_counts_with_wide_tables(N):
+    run([130, 0, 700], N, 8, 2, 64, 64, seed=N, width=WIDE)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(3, 1), (24, 8), (16, 1), (32, 8), (10, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_head_layouts_with_wide_tables(Hq, Hkv, D):
+    run([200, 65, 1], -(-33 * Hkv // Hq), Hq, Hkv, D, 32, seed=Hq, width=4 * WIDE)
+
+
+@pytest.mark.parametrize("kind", ["chain", "star", "ragged"])
+@pytest.mark.parametrize("N,Hq", [(12, 8), (50, 4), (128, 2)])
+def test_tree_shapes_with_wide_tables(kind, N, Hq):
+    run([0, 90, 400], N, Hq, 2, 64, 64, kind=kind, seed=N, width=WIDE)
 
 
 def test_batch_of_many():
