@@ -485,8 +485,8 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split, and
  * counters: it must be zero before its first use; calls leave them zero (one workspace
  * may serve calls of the same sizes that do not overlap on the GPU).
- * From 33 rows (nodes x Hq / kv_heads) per kv head on it runs on the tcgen05 tensor cores;
- * iron_tree_attn_status returns IRON_ERR_TIMEOUT if a bounded wait ran out there since the
+ * With more than 32 rows (nodes x Hq / kv_heads) per kv head it may run on the tcgen05 tensor
+ * cores; iron_tree_attn_status returns IRON_ERR_TIMEOUT if a bounded wait ran out there since the
  * last reset (reset != 0 clears it); it synchronises the device. */
 int iron_tree_attn_status(int reset);
 size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
