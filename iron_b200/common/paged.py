@@ -117,20 +117,17 @@ def address(t):
 _stride_arrays: dict = {}
 
 
-def stride_array(strides):
-    """The strides as an int64 array for the C entry points (made once per set of strides)."""
-    a = _stride_arrays.get(strides)
+def stride_array(t, shape):
+    """Element strides of the leading dimensions of `t` seen as `shape`, as an int64 array for
+    the C entry points (made once per set of strides, so equal strides give the same array)."""
+    full = t.stride()
+    if t.shape != shape:
+        full, step = [1], 1
+        for n in reversed(shape[1:]):
+            step *= n
+            full.append(step)
+        full = tuple(reversed(full))
+    a = _stride_arrays.get(full)
     if a is None:
-        a = _stride_arrays[strides] = (ctypes.c_int64 * len(strides))(*strides)
+        a = _stride_arrays[full] = (ctypes.c_int64 * (len(full) - 1))(*full[:-1])
     return a
-
-
-def strides(t, shape):
-    """Element strides of the leading dimensions of `t` seen as `shape`."""
-    if t.shape == shape:
-        return t.stride()[:-1]
-    out, step = [], 1
-    for n in reversed(shape[1:]):
-        step *= n
-        out.append(step)
-    return tuple(reversed(out))

@@ -26,7 +26,7 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, address, stride_array, strides
+from ...common.paged import PagedOperator, address, stride_array
 from ...common.verify import Tolerance
 
 
@@ -77,7 +77,7 @@ class PageSelectAttention(PagedOperator):
                              self.num_pages, self.max_pages, self.num_kv_heads, self.head_dim, self.page_size)
         scale = 1.0 / math.sqrt(self.head_dim) if self.scale is None else self.scale
         _lib.call("iron_page_select_attn", ctypes.byref(pool), p(q), p(out), p(selected), self.num_heads,
-                  self.top_pages, stride_array(strides(q, rows)), stride_array(strides(out, rows)), scale, ws, nbytes, flags, stream)
+                  self.top_pages, stride_array(q, rows), stride_array(out, rows), scale, ws, nbytes, flags, stream)
 
     def reference(self, q, k_pages, v_pages, codes, scales, page_table, lens):
         """(out, selected) by the rule, head by head."""

@@ -27,7 +27,7 @@ import numpy as np
 
 from ... import _lib
 from ...common.base import AIERuntimeArgSpec
-from ...common.paged import PagedOperator, address, stride_array, strides
+from ...common.paged import PagedOperator, address, stride_array
 from ...common.verify import Tolerance
 
 
@@ -74,15 +74,15 @@ class TreeAttention(PagedOperator):
         p = address
         new = (self.batch, self.num_nodes, self.num_kv_heads, self.head_dim)
         rows = (self.batch, self.num_nodes, self.num_heads, self.head_dim)
-        ks = strides(k_new, new)
-        if strides(v_new, new) != ks:
+        ks = stride_array(k_new, new)
+        if stride_array(v_new, new) is not ks:
             raise ValueError("k_new and v_new must have the same strides")
         ws, nbytes = self._workspace(stream)
         pool = _lib.PagePool(p(k_pages), p(v_pages), None, None, p(page_table), p(lens), None, 1, self.batch,
                              self.num_pages, self.max_pages, self.num_kv_heads, self.head_dim, self.page_size)
         scale = 1.0 / math.sqrt(self.head_dim) if self.scale is None else self.scale
         _lib.call("iron_tree_attn", ctypes.byref(pool), p(q), p(k_new), p(v_new), p(parents), p(out), self.num_nodes,
-                  self.num_heads, stride_array(strides(q, rows)), stride_array(ks), stride_array(strides(out, rows)), scale, ws,
+                  self.num_heads, stride_array(q, rows), ks, stride_array(out, rows), scale, ws,
                   nbytes, flags, stream)
 
     def reference(self, q, k_new, v_new, k_pages, v_pages, page_table, lens, parents):
