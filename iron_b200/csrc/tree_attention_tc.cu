@@ -23,7 +23,8 @@
 // (measured alone: S of 64 columns 48 cycles per MMA, of 128 columns 62; P V 33 and 60).
 // 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 107 us, D = 128 120; without the
 // MMAs 100, without ex2 88, without all arithmetic of the softmax 71 (D = 64): no unit is
-// full, and the chain from S through TMEM and registers to P sets the pace. 8 sequences of
+// full (issue 40 %, ex2 36 %, tensor 27 %); the 550 instructions of a warp per 64 tokens, with
+// two such warps per scheduler, set the pace. 8 sequences of
 // 32768 tokens, D = 128: 282 us, tensor cores 70 % busy (335 in long runs, at the power
 // limit). What a tile must not hold (past the length, unused nodes) is masked in S and
 // zeroed in V.
@@ -570,7 +571,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             by = 1.f;
           }
           const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), minus = pack2(-1.f, -1.f);
-          uint64_t sum[2] = {0, 0};
+          uint64_t sum[4] = {0, 0, 0, 0};
           uint32_t hi[32], lo[32];
 #pragma unroll
           for (int q = 0; q < 32; ++q) {
@@ -579,7 +580,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             p0 = ex2_approx(p0);
             p1 = ex2_approx(p1);
             const uint64_t p = pack2(p0, p1);
-            sum[q & 1] = add2(sum[q & 1], p);
+            sum[q & 3] = add2(sum[q & 3], p);
             hi[q] = pack_bf16x2(p0, p1);
             unpack2(fma2(pack2(bf16_lo(hi[q]), bf16_hi(hi[q])), minus, p), p0, p1);
             lo[q] = pack_bf16x2(p0, p1);
@@ -601,7 +602,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           tc::arrive_if(lane == 0, bars.pfull<S>(s));
           ++vc;
           float s0, s1;
-          unpack2(add2(sum[0], sum[1]), s0, s1);
+          unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
           l += s0 + s1;
         }
       }
