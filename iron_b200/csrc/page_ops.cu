@@ -341,7 +341,6 @@ struct ForkArgs {
   int *table_out, *lens_out, *refs_out, *status;
   int *fresh;          // workspace [S]: the page a slot's partial page is copied to, or -1
   int *from;           // workspace [S]: the old slot, or -1
-  int *list;           // workspace [S]: free pages
   int4 *copies;        // workspace [S]: {old page, new page, rows} of the partial pages to copy
   int *count;          // workspace [1]
   int64_t layer_stride;
@@ -350,7 +349,7 @@ struct ForkArgs {
 
 // Block 0 plans; the others copy the reference counts to refs_out.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
-  __shared__ int src[kMaxSlots], keeper[kMaxSlots], length[kMaxSlots];
+  __shared__ int src[kMaxSlots], keeper[kMaxSlots], length[kMaxSlots], list[kMaxSlots];
   __shared__ int warp_sums[32], counts[257], refused;
   pdl_launch_dependents();
   pdl_wait();
@@ -371,35 +370,34 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   for (int s = threadIdx.x; s < a.S; s += kPlanThreads)
     if (src[s] >= 0) atomicMin(&keeper[src[s]], src[s] == s ? -1 : s);
   __syncthreads();
-  int before = 0;
-  for (int s0 = 0; s0 < a.S; s0 += kPlanThreads) {
-    const int s = s0 + threadIdx.x;
-    const int r = s < a.S ? src[s] : -1;
+  // a slot's rank among those that copy, and the page that it copies from: requested before
+  // the free pages are looked for
+  constexpr int kPer = kMaxSlots / kPlanThreads;
+  int rank[kPer], from[kPer], before = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = i * kPlanThreads + threadIdx.x, r = s < a.S ? src[s] : -1;
     const bool copy = r >= 0 && length[r] % a.page > 0 && r != s && keeper[r] != s;
-    int sum;
-    const int rank = block_scan(copy ? 1 : 0, warp_sums, &sum) - 1;
-    if (s < a.S) {
-      a.fresh[s] = copy ? before + rank : -1;  // the rank, until the pages are known
-      a.from[s] = r;
-    }
+    from[i] = copy ? ld_act_i32(a.table + static_cast<int64_t>(r) * a.M + length[r] / a.page) : -1;
+    int sum = 0;
+    if (i * kPlanThreads < a.S) rank[i] = before + block_scan(copy ? 1 : 0, warp_sums, &sum) - 1;
+    if (!copy) rank[i] = -1;
     before += sum;
   }
-  const int got = collect_pages(a.refs, 0, a.P, false, before, a.list, counts);
+  const int got = collect_pages(a.refs, 0, a.P, false, before, list, counts);
   __syncthreads();
-  for (int s = threadIdx.x; s < a.S; s += kPlanThreads) {
-    const int rank = a.fresh[s];
-    const bool off = rank >= got;  // no page left: the slot stays empty
-    if (rank >= 0) a.fresh[s] = off ? -1 : a.list[rank];
-    if (off) {
-      a.from[s] = -1;
-      atomicAdd(&refused, 1);
-    }
-    if (rank >= 0 && !off) {
-      const int len = length[src[s]], p = ld_act_i32(a.table + static_cast<int64_t>(src[s]) * a.M + len / a.page);
-      // a table entry that is no page of the pool: nothing to copy
-      a.copies[rank] = make_int4(p, a.list[rank], p >= 0 && p < a.P ? len % a.page : 0, 0);
-    }
-    a.lens_out[s] = src[s] >= 0 && !off ? length[src[s]] : 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = i * kPlanThreads + threadIdx.x;
+    if (s >= a.S) break;
+    const bool off = rank[i] >= got;  // no page left: the slot stays empty
+    const int to = rank[i] >= 0 && !off ? list[rank[i]] : -1, len = src[s] >= 0 && !off ? length[src[s]] : 0;
+    a.fresh[s] = to;
+    a.from[s] = off ? -1 : src[s];
+    a.lens_out[s] = len;
+    if (off) atomicAdd(&refused, 1);
+    // a table entry that is no page of the pool: nothing to copy
+    if (to >= 0) a.copies[rank[i]] = make_int4(from[i], to, from[i] >= 0 && from[i] < a.P ? len % a.page : 0, 0);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -629,7 +627,7 @@ extern "C" int iron_page_append(const iron_page_pool *c, const uint16_t *k_new, 
 }
 
 extern "C" size_t iron_page_fork_workspace_bytes(int slots) {
-  return slots > 0 ? static_cast<size_t>(slots) * 7 * sizeof(int) + 16 : 0;
+  return slots > 0 ? static_cast<size_t>(slots) * 6 * sizeof(int) + 16 : 0;
 }
 
 extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, int32_t *page_table_out,
@@ -658,8 +656,7 @@ extern "C" int iron_page_fork(const iron_page_pool *c, const int32_t *source, in
   a.copies = static_cast<int4 *>(workspace);
   a.fresh = reinterpret_cast<int *>(a.copies + c->slots);
   a.from = a.fresh + c->slots;
-  a.list = a.from + c->slots;
-  a.count = a.list + c->slots;
+  a.count = a.from + c->slots;
   a.layers = c->layers;
   a.S = c->slots;
   a.Hkv = c->kv_heads;
