@@ -175,6 +175,24 @@ def test_tree_shapes_with_wide_tables(kind, N, Hq):
     run([0, 90, 400], N, Hq, 2, 64, 64, kind=kind, seed=N, width=WIDE)
 
 
+@pytest.mark.parametrize("width", [16, 3000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_broadcast_rows_and_other_scales(D, width):
+    """Keys of one batch for all sequences (stride 0), and a scale below zero: many rows
+    without the tensor cores' form."""
+    cache = Cache([70, 0, 900, 130], 2, D, 64, 5, width=width)
+    rng, g = random.Random(2), gen(5)
+    N, Hq, scale = 40, 8, -0.07
+    q = randn(g, 4, N, Hq, D)
+    kn, vn = (randn(g, 1, N, 2, D).expand(4, N, 2, D) for _ in range(2))
+    parents = [drafted(rng, "ragged", N) for _ in range(4)]
+    table = torch.tensor(parents, dtype=torch.int32, device="cuda")
+    for k, v, x in ((kn, vn, None), (kn.contiguous(), vn.contiguous(), scale)):
+        out = torch.full_like(q, math.nan)
+        operator(cache, 4, N, Hq, x).get_callable()(q, k, v, cache.k, cache.v, cache.table, cache.lens, table, out)
+        close(out, *tree_reference(cache, q, k, v, parents, x or 1 / math.sqrt(D)))
+
+
 def test_batch_of_many():
     rng = random.Random(2)
     run([rng.randint(0, 200) for _ in range(300)], 2, 4, 1, 64, 32, seed=2)
