@@ -425,6 +425,8 @@ int iron_attn_prefill(const uint16_t *q, const uint16_t *k, const uint16_t *v, u
  *   refs     int32 [num_pages]: how many table rows hold the page (0: free).
  * head_dim 64 or 128; page_size 16, 32, 64 or 128; page * max_pages < 2^31; pools and
  * codes 16-byte aligned. Table entries outside [0, num_pages) are never followed.
+ * Tables, lengths and counts are read on the device, by several CTAs each for itself: nothing
+ * may write them while a call runs (a writer on another stream needs an event in between).
  * These entry points read nothing before they have waited for the stream's previous
  * kernel, so they always launch the way IRON_FLAG_PDL asks for; the flag changes nothing.
  *
