@@ -375,10 +375,10 @@ extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int n
 // where the form above would need a second unit of 32; but up to kFewRows rows only if full
 // tables hold more than kFewTiles tiles of 16 rows: that form's pipeline takes about 13 us
 // (head dim 64) or 18 (128) to fill and drain. B200, us, here / there: 32 rows, 16 x 4608 tokens
-// at head dim 64 49 / 60, 8 x 32768 at 128 231 / 296; 36 rows 74 / 60 and 422 / 296; 64 rows,
-// 1 x 300 (160 tiles) 9.9 / 13.5, 1 x 4608 (2304) 21 / 22 and at 128 30 / 40, 4 x 4608 (9216)
-// 32 / 27 and 55 / 41; 104 rows, 1 x 2304 (2016) 19 / 20 and 28 / 36; 256 rows, 1 x 300 at 128
-// (640) 26 / 21.
+// at head dim 64 49 / 62, 64 x 2304 87 / 130, 8 x 32768 at 128 230 / 310; 36 rows 74 / 62, 154 / 132
+// and 437 / 309; 64 rows, 1 x 300 (160 tiles) 11 / 14, 1 x 4608 (2304) 22 / 23 and at 128 32 / 41,
+// 4 x 4608 (9216) 35 / 27 and 57 / 44; 104 rows, 1 x 2304 (2016) 19 / 20 and 28 / 36; 256 rows,
+// 1 x 300 at 128 (640) 26 / 21.
 constexpr int kTensorRows = 33, kFewRows = 128, kFewTiles = 2560;
 
 // The tcgen05 form takes positive scales that do not vanish in log2 units, and new rows

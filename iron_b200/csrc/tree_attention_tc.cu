@@ -21,8 +21,8 @@
 // Bounds (B200): per 128 tokens and stream 1024 cycles of ex2 (16 per cycle and SM for 128
 // rows), and on the tensor cores 250 of S and 530 of P V at D = 64, 770 and 960 at D = 128
 // (measured alone: S of 64 columns 48 cycles per MMA, of 128 columns 62; P V 33 and 60).
-// 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 107 us, D = 128 120; without the
-// MMAs 100, without ex2 88, without all arithmetic of the softmax 71 (D = 64): no unit is
+// 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 112 us, D = 128 131 (of 107 at D =
+// 64: without the MMAs 100, without ex2 88, without all arithmetic of the softmax 71): no unit is
 // full (issue 40 %, ex2 36 %, tensor 27 %); the 550 instructions of a warp per 64 tokens, with
 // two such warps per scheduler, set the pace. 8 sequences of
 // 32768 tokens, D = 128: 282 us, tensor cores 70 % busy (335 in long runs, at the power
@@ -305,13 +305,24 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     } else if (warp < 10) {
       // ---- MMAs of stream `s`: the warp stays converged, an elected lane issues. (One warp for
       // both streams was what bound the kernel: its instructions share their scheduler with
-      // two softmax warps, and each stream waited for the other one's turn.) ----
+      // two softmax warps, and each stream waited for the other one's turn.) A wait names a
+      // phase by its parity alone, so neither stream may get two phases away from a slot: each
+      // goes through all tiles in order, and waits for and releases those of the other too. ----
       const int s = warp - 8;
       constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kTile, C::kScores);
       constexpr uint32_t idesc_o = tc::idesc_bf16_f32(kTile, D) | (1u << 16);  // B (V) is MN-major
       bool ok = true;
       int it0 = 0;
+      bool owed = false;  // V of the last segment's last tile is still to be released
       uint32_t pc = 0, qc = 0, sn = 0;
+      auto pass_k = [&](int it) {
+        ok &= wait_phase(bars.kfull<S>(it % S), (it / S) & 1);
+        tc::arrive_if(lane == 0, bars.kempty<S>(it % S));
+      };
+      auto pass_v = [&](int it) {
+        ok &= wait_phase(bars.vready<S>(it % S), (it / S) & 1);
+        tc::arrive_if(lane == 0, bars.vempty<S>(it % S));
+      };
       for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); uniform(sg.count) > 0;
            sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
         const Streams st = streams_of(a, sg);
@@ -319,12 +330,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         const int first = uniform(sg.first), n = uniform(st.n[s]);
         const bool both = uniform(st.both);
         const int it0s = it0 + (both ? 0 : s), step = both ? 1 : 2;
-        // K and V are released by both streams; a tile that one stream has alone, by it twice
-        const bool twice = !both;
         auto halves = [&](int j) { return halves_of(a, first + (both ? j : 2 * j + s), ctiles, len); };
         // S of tile j: all of it (h = 0), or its half h
         auto scores = [&](int j, int h, bool last) {
           const int it = it0s + j * step, slot = it % S;
+          if (!both && h == 0 && it > it0) pass_k(it - 1);
           ok &= wait_phase(bars.kfull<S>(slot), (it / S) & 1);
           if (sn > 0) ok &= wait_phase(bars.sfree<S>(s), (sn - 1) & 1);
           ++sn;
@@ -340,15 +350,13 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
                 tc::mma_bf16(tmem + C::kTmemS + s * C::kScores, q + c * (C::kPanel >> 4) + kk * 2,
                              k + c * (C::kPanel >> 4) + kk * 2, idesc_s, c > 0 || kk > 0);
             tc::mma_commit(bars.sfull<S>(s));
-            if (last) {
-              tc::mma_commit(bars.kempty<S>(slot));
-              if (twice) tc::mma_commit(bars.kempty<S>(slot));
-            }
+            if (last) tc::mma_commit(bars.kempty<S>(slot));
           }
           __syncwarp();
         };
         auto values = [&](int j, int h, bool last) {
           const int it = it0s + j * step, slot = it % S;
+          if (!both && h == 0 && it > it0) pass_v(it - 1);
           ok &= wait_phase(bars.vready<S>(slot), (it / S) & 1);
           ok &= wait_phase(bars.pfull<S>(s), pc++ & 1);
           tc::fence_after_sync();
@@ -361,10 +369,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
               for (int kk = 0; kk < 4; ++kk)
                 tc::mma_bf16_ts(o, p + part * 32 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || h > 0 || part > 0 || kk > 0);
             tc::mma_commit(bars.pvdone<S>(s));
-            if (last) {
-              tc::mma_commit(bars.vempty<S>(slot));
-              if (twice) tc::mma_commit(bars.vempty<S>(slot));
-            }
+            if (last) tc::mma_commit(bars.vempty<S>(slot));
           }
           __syncwarp();
         };
@@ -372,6 +377,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           ok &= wait_phase(bars.qfull<S>(s), qc++ & 1);
           int k = halves(0);
           scores(0, 0, C::kScores == kTile || k == 1);
+          if (owed) pass_v(it0 - 1);
+          owed = false;
           // the S that follows goes out before the P V of the last half that the present S
           // holds: it runs while that half's softmax does, and the softmax never waits for it
           for (int j = 0; j < n; ++j) {
@@ -386,8 +393,15 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             if (!ok) break;
           }
         }
-        if (!ok) break;
         it0 += uniform(sg.count);
+        if (!both && ((sg.count - 1) & 1) != s) {  // the last tile is the other stream's
+          pass_k(it0 - 1);
+          // its V once the next segment's first K is on its way
+          if (owed) pass_v(it0 - 2);
+          owed = true;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
       if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
       // every MMA issued is done before TMEM is freed
