@@ -488,9 +488,13 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * counters: it must be zero before its first use; calls leave them zero (one workspace
  * may serve calls of the same sizes that do not overlap on the GPU).
  * With more than 32 rows (nodes x Hq / kv_heads) per kv head it may run on the tcgen05 tensor
- * cores; iron_tree_attn_status returns IRON_ERR_TIMEOUT if a bounded wait ran out there since the
- * last reset (reset != 0 clears it); it synchronises the device. */
+ * cores, whose waits are bounded: a call in which one runs out ends, and leaves rows unwritten.
+ * iron_tree_attn_status synchronises the device and returns IRON_ERR_TIMEOUT if that happened on
+ * it since the last reset (reset != 0 clears it). A wait ends after 2 s, and when another one of
+ * the block has run out; iron_tree_attn_set_wait_us sets, for the calls that follow, how long a
+ * block's loads wait for room (0: not at all, so every call of more than a few tiles ends so). */
 int iron_tree_attn_status(int reset);
+int iron_tree_attn_set_wait_us(unsigned limit_us);
 size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
 int iron_tree_attn(const iron_page_pool *pool, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
                    const int32_t *parents, uint16_t *out, int num_nodes, int num_heads, const int64_t *q_strides,

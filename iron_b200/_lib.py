@@ -89,6 +89,7 @@ SIGNATURES: dict[str, list] = {
     "iron_tree_attn_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
     "iron_tree_attn": [P, P, P, P, P, P, c_int, c_int, P, P, P, c_float, P, c_size_t, c_uint, P],
     "iron_tree_attn_status": [c_int],
+    "iron_tree_attn_set_wait_us": [c_uint],
     "iron_page_select_attn_workspace_bytes": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
     "iron_page_select_attn": [P, P, P, P, c_int, c_int, P, P, c_float, P, c_size_t, c_uint, P],
     "iron_attn_prefill": [P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P, P, c_float, c_int,

@@ -143,7 +143,7 @@ class PagedDecoder:
     def verify(self, tokens, parents):
         """tokens, parents int32 [slots, nodes] (device): the model's predictions after each node,
         int32 [slots, nodes]; `logits` holds the rows. The nodes' keys and values are kept
-        for `accept`."""
+        for `accept`. Nothing waits for the GPU; `check` does, and raises if the attention gave up."""
         c, B, N = self.cache, self.slots, self.nodes
         G, D = self.s.n_kv_groups, self.s.head_dim
         depth = torch.zeros(B, N, **self._ints)
@@ -160,6 +160,12 @@ class PagedDecoder:
                        out.view(B, N, -1, D))
 
         return self._forward(tokens.reshape(-1), positions, attend).view(B, N)
+
+    def check(self):
+        """Waits for the GPU and raises RuntimeError if the cache refused a slot or a tree attention
+        gave up a bounded wait since the last check."""
+        TreeAttention.check()
+        self.cache.check()
 
     def accept(self, paths):
         """Appends the listed nodes of the last `verify` to their slots (an empty list: none)."""
@@ -190,6 +196,7 @@ class PagedDecoder:
             drafts += [([0] * N, [-2] * N)] * (self.slots - len(texts))
             tokens, parents = (torch.tensor([d[i] for d in drafts], dtype=torch.int32, device=dev) for i in (0, 1))
             predicted = self.verify(tokens, parents).tolist()
+            TreeAttention.check()
             self.passes += 1
             paths = [[]] * self.slots
             for i, t in enumerate(texts):

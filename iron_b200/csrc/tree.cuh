@@ -18,6 +18,7 @@ struct TreeArgs {
   int64_t qs[3], ks[3], os[3];  // element strides {batch, node, head}
   int B, N, Hq, Hkv, groups /* row groups per (sequence, kv head) */, page_shift, M, P;
   float scale_log2;
+  unsigned wait_us;  // how long the loads of the tcgen05 form wait for room
 };
 
 __device__ __forceinline__ int cached_len(const TreeArgs &a, int b) {
@@ -196,5 +197,6 @@ static_assert(kTMaxNodes == 128, "four words of 32 nodes");
 // The tcgen05 form (tree_attention_tc.cu).
 size_t tree_tc_workspace(int head_dim);
 int tree_tc_launch(TreeArgs a, int head_dim, cudaStream_t s);
+unsigned tree_wait_us();  // the limit that iron_tree_attn_set_wait_us set
 
 }  // namespace iron

@@ -450,6 +450,7 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.M = c->max_pages;
   a.P = c->num_pages;
   a.scale_log2 = scale * kLog2e;
+  a.wait_us = tree_wait_us();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (use_tensor_form(a, tiles)) return tree_tc_launch(a, c->head_dim, s);
   const bool two = unit == 32;

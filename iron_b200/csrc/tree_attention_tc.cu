@@ -31,6 +31,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "tc.cuh"
 #include "tree.cuh"
 
@@ -54,9 +56,10 @@ struct Cut {
 };
 constexpr int kMasks = 8;  // tiles' masks in flight: stages + 2 at least
 
-// Bounded wait for a barrier phase: false after 2 s. The clock is read every 256 polls
-// only, which waits of the usual length never reach.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+// Bounded wait for a barrier phase: false after limit_us, or once *stop is set (some role
+// gave up, so what it owes the others will not come). Both are looked at every 256 polls only,
+// which waits of the usual length never reach.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int *stop, uint32_t limit_us = 2000000) {
   uint64_t start = 0;
   for (uint32_t i = 1;; ++i) {
     uint32_t done;
@@ -69,11 +72,25 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
         : "memory");
     if (done) return true;
     if ((i & 255u) == 0u) {
+      if (stop && *stop) return false;
       const uint64_t now = tc::globaltimer_ns();
       if (start == 0) start = now;
-      else if (now - start > 2000000000ull) return false;
+      else if (now - start > limit_us * 1000ull) return false;
     }
   }
+}
+// The loads' wait for room, whose limit the caller sets; a limit of 0 looks once.
+__device__ __forceinline__ bool wait_room(uint32_t bar, uint32_t parity, const volatile int *stop, uint32_t limit_us) {
+  if (limit_us > 0) return wait_phase(bar, parity, stop, limit_us);
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done;
 }
 
 template <int D>
@@ -176,11 +193,18 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
   __shared__ TreePaths trees[C::kTrees];
   __shared__ float2 other_ml[kTile];        // (m, l) of stream 1, for the join of both streams
   __shared__ int odd_flag;                  // V of the tree held values that are not finite
+  __shared__ int stop;                      // a wait ran out
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *smem = smem_raw + (base - raw);
   const uint32_t q0 = base, k0 = base + 2 * C::kOperand, v0 = k0 + S * C::kOperand;
   const Bars bars{smem_addr(bar_store)};
+  auto wait_phase = [&](uint32_t bar, uint32_t parity) { return treetc::wait_phase(bar, parity, &stop); };
+  auto drain = [&](uint32_t bar, uint32_t parity) { treetc::wait_phase(bar, parity, nullptr); };  // what is in flight
+  auto give_up = [&](unsigned role) {
+    *const_cast<volatile int *>(&stop) = 1;
+    atomicCAS(&g_tree_status, 0u, role);
+  };
 
   pdl_launch_dependents();
   pdl_wait();
@@ -211,6 +235,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
     tc::mbar_init_u32(bars.other<S>(), 4);
     tc::mbar_init_u32(bars.joined<S>(), 4);
     odd_flag = 0;
+    stop = 0;
     mbar_init_fence();
   }
   if (warp == 8) tc::tmem_alloc(smem_addr(&tmem_slot), 512);
@@ -230,7 +255,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       }
       const int page = 1 << a.page_shift, ppt = kTile >> a.page_shift;  // pages per tile
       bool ok = true;
-      int it = 0;
+      int it = 0, sent_v = 0;  // tiles whose K and V are on their way or there
       for (Segment sg = next_segment<Cut>(a, pref, w_begin, w_end); sg.count > 0 && ok;
            sg = next_segment<Cut>(a, pref, sg.next, w_end)) {
         const int len = cached_len(a, sg.b), ctiles = (len + kTile - 1) / kTile;
@@ -242,7 +267,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           return e < a.M ? ld_act_i32(table + e) : -1;
         };
         int cur = entries(sg.first), next = entries(sg.first + per), used = 0;
-        for (int i = sg.first; i < sg.first + sg.count; ++i, ++it) {
+        for (int i = sg.first; i < sg.first + sg.count; ++i) {
           const int s = it % S;
           const bool tree = i >= ctiles;
           // this tile's pages: lane l < ppt holds page l and its valid rows
@@ -264,7 +289,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, n > 0));
           const uint32_t bytes = tree ? C::kOperand : boxes * page * D * 2;
           const uint32_t parity = ((it / S) & 1) ^ 1;
-          ok = __all_sync(0xffffffffu, wait_phase(bars.kempty<S>(s), parity));
+          ok = __all_sync(0xffffffffu, wait_room(bars.kempty<S>(s), parity, &stop, a.wait_us));
           if (!ok) break;
           if (lane < 4) masks[it % kMasks][lane] = bits;
           __syncwarp();
@@ -283,24 +308,20 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             }
           };
           load(&maps.k, &maps.k_new, k0 + s * C::kOperand, bars.kfull<S>(s));
-          ok = __all_sync(0xffffffffu, wait_phase(bars.vempty<S>(s), parity));
-          if (!ok) {
-            // this tile's K is on its way already: let it land
-            wait_phase(bars.kfull<S>(s), (it / S) & 1);
-            break;
-          }
+          ++it;
+          ok = __all_sync(0xffffffffu, wait_room(bars.vempty<S>(s), parity, &stop, a.wait_us));
+          if (!ok) break;
           if (lane == 0) tc::expect_tx(bars.vfull<S>(s), bytes);
           __syncwarp();
           load(&maps.v, &maps.v_new, v0 + s * C::kOperand, bars.vfull<S>(s));
+          sent_v = it;
         }
       }
       if (!ok) {
-        if (lane == 0) atomicCAS(&g_tree_status, 0u, 1u);
+        if (lane == 0) give_up(1);
         // copies in flight land before the CTA's shared memory goes away
-        for (int j = max(0, it - S); j < it; ++j) {
-          wait_phase(bars.kfull<S>(j % S), (j / S) & 1);
-          wait_phase(bars.vfull<S>(j % S), (j / S) & 1);
-        }
+        for (int j = max(0, it - S); j < it; ++j) drain(bars.kfull<S>(j % S), (j / S) & 1);
+        for (int j = max(0, sent_v - S); j < sent_v; ++j) drain(bars.vfull<S>(j % S), (j / S) & 1);
       }
     } else if (warp < 10) {
       // ---- MMAs of stream `s`: the warp stays converged, an elected lane issues. (One warp for
@@ -403,11 +424,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 2u);
+      if (!ok && lane == 0) give_up(2);
       // every MMA issued is done before TMEM is freed
       if (tc::elect_one()) tc::mma_commit(bars.drain<S>(s));
       __syncwarp();
-      wait_phase(bars.drain<S>(s), 0);
+      drain(bars.drain<S>(s), 0);
       __syncwarp();
     } else {
       // ---- preparation: warp 11 ----
@@ -461,7 +482,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
           tc::arrive_if(lane == 0, bars.vready<S>(slot));
         }
       }
-      if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 5u);
+      if (!ok && lane == 0) give_up(5);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -712,7 +733,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
       sg = next;
       st = nst;
     }
-    if (!ok && lane == 0) atomicCAS(&g_tree_status, 0u, 3u + s);
+    if (!ok && lane == 0) give_up(3u + s);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -835,7 +856,18 @@ int tree_tc_launch(TreeArgs a, int head_dim, cudaStream_t s) {
 
 }  // namespace iron
 
+static std::atomic<unsigned> g_tree_wait_us{2000000};
+
+unsigned iron::tree_wait_us() { return g_tree_wait_us.load(std::memory_order_relaxed); }
+
+extern "C" int iron_tree_attn_set_wait_us(unsigned limit_us) {
+  g_tree_wait_us.store(limit_us, std::memory_order_relaxed);
+  return IRON_OK;
+}
+
 extern "C" int iron_tree_attn_status(int reset) {
+  // the copies below run on the default stream, which other streams need not wait for
+  if (cudaDeviceSynchronize() != cudaSuccess) return iron::launch_status();
   unsigned v = 0;
   if (cudaMemcpyFromSymbol(&v, iron::g_tree_status, sizeof(v)) != cudaSuccess) return iron::launch_status();
   if (reset) {

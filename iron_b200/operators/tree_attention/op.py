@@ -15,6 +15,8 @@ num_nodes]; out bf16 like q.
 parents[b, i] is -1 (a child of the cached prefix) or a node j < i. Any other value marks an
 unused place; a node below an unused one is unused too. Unused rows give zeros, and nothing
 that a node's path does not hold reaches its row, whatever its values.
+
+The kernel for many rows waits with a limit; ``check`` raises if a wait ran out.
 """
 
 from __future__ import annotations
@@ -84,6 +86,15 @@ class TreeAttention(PagedOperator):
         _lib.call("iron_tree_attn", ctypes.byref(pool), p(q), p(k_new), p(v_new), p(parents), p(out), self.num_nodes,
                   self.num_heads, stride_array(q, rows), ks, stride_array(out, rows), scale, ws,
                   nbytes, flags, stream)
+
+    @staticmethod
+    def check():
+        """Waits for the GPU and raises RuntimeError if a bounded wait ran out in a tree attention
+        on the current device since the last check: outputs of the calls in between are not whole."""
+        status = _lib.load().iron_tree_attn_status(1)
+        if status == _lib.IRON_ERR_TIMEOUT:
+            raise RuntimeError("TreeAttention: a bounded wait timed out, the outputs are not whole")
+        _lib.check(status, "iron_tree_attn_status")
 
     def reference(self, q, k_new, v_new, k_pages, v_pages, page_table, lens, parents):
         """The formula, row by row, in fp32."""
