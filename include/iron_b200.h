@@ -71,6 +71,9 @@ const char *iron_strerror(int status);
 int iron_last_cuda_error(void);
 /* ABI version: (major << 16) | minor. */
 int iron_abi_version(void);
+/* *id = the id of the capture that `stream` is part of (a different one for each CUDA graph that
+ * is captured), 0 if it is not captured. */
+int iron_capture_id(void *stream, unsigned long long *id);
 
 /* ---- GEMV (bf16 weights) --------------------------------------------------
  * Replaces GEMV(M, K, num_batches, epilogue) -- iron/operators/gemv/op.py:22-159,
@@ -484,9 +487,10 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * its values. q, out bf16 [batch, num_nodes, Hq, D], k_new, v_new bf16 [batch, num_nodes,
  * kv_heads, D] with element strides {batch, node, head} (3 int64 each, multiples of 8; kv
  * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024.
- * `workspace` >= iron_tree_attn_workspace_bytes holds the partials of what is split, and
- * counters: it must be zero before its first use; calls leave them zero (one workspace
- * may serve calls of the same sizes that do not overlap on the GPU).
+ * `workspace` >= iron_tree_attn_workspace_bytes holds counters, in its first
+ * iron_tree_attn_counter_bytes, and the partials of what is split. The counters must be zero
+ * before the first use; calls leave them zero (one workspace may serve calls of the same sizes
+ * that do not overlap on the GPU; a captured graph may replay beside any call, so it needs its own).
  * With more than 32 rows (nodes x Hq / kv_heads) per kv head it may run on the tcgen05 tensor
  * cores, whose waits are bounded: a call in which one runs out ends, and leaves rows unwritten.
  * iron_tree_attn_status synchronises the device and returns IRON_ERR_TIMEOUT if that happened on
@@ -495,6 +499,7 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * block's loads wait for room (0: not at all, so every call of more than a few tiles ends so). */
 int iron_tree_attn_status(int reset);
 int iron_tree_attn_set_wait_us(unsigned limit_us);
+size_t iron_tree_attn_counter_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
 size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim);
 int iron_tree_attn(const iron_page_pool *pool, const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
                    const int32_t *parents, uint16_t *out, int num_nodes, int num_heads, const int64_t *q_strides,

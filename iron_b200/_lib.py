@@ -33,6 +33,7 @@ SIGNATURES: dict[str, list] = {
     "iron_strerror": [c_int],
     "iron_last_cuda_error": [],
     "iron_abi_version": [],
+    "iron_capture_id": [P, P],
     "iron_gemv_bf16": [P, P, P, c_int, c_int, c_int64, c_int, c_int64, c_int64, c_int64,
                        c_int, P, c_int, c_uint, P],
     "iron_pack_int4g32": [P, P, P, c_int, c_int, P],
@@ -87,6 +88,7 @@ SIGNATURES: dict[str, list] = {
     "iron_page_compact_workspace_bytes": [c_int],
     "iron_page_compact": [P, P, P, P, P, c_size_t, c_uint, P],
     "iron_tree_attn_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "iron_tree_attn_counter_bytes": [c_int, c_int, c_int, c_int, c_int],
     "iron_tree_attn": [P, P, P, P, P, P, c_int, c_int, P, P, P, c_float, P, c_size_t, c_uint, P],
     "iron_tree_attn_status": [c_int],
     "iron_tree_attn_set_wait_us": [c_uint],
@@ -102,6 +104,7 @@ _RESTYPES = {"iron_strerror": c_char_p, "iron_attn_decode_workspace_bytes": c_si
              "iron_page_fork_workspace_bytes": c_size_t,
              "iron_page_compact_workspace_bytes": c_size_t,
              "iron_tree_attn_workspace_bytes": c_size_t,
+             "iron_tree_attn_counter_bytes": c_size_t,
              "iron_page_select_attn_workspace_bytes": c_size_t}
 
 class GemvChain(ctypes.Structure):

@@ -25,8 +25,11 @@ PAGE_SIZES = (16, 32, 64, 128)
 
 
 class PagedOperator(MLIROperator):
-    """Checks each buffer's device, type, size and order, and keeps one workspace per stream
-    (calls on different streams may overlap; calls on one stream follow one another)."""
+    """Checks each buffer's device, type, size and order, and keeps one workspace per device and
+    stream (calls on different streams may overlap; calls on one stream follow one another).
+
+    A CUDA graph may replay on any stream, beside anything, so the calls that it captures have a
+    workspace of the graph's own (one per captured stream), taken from the graph's memory."""
 
     def _check_geometry(self):
         if self.head_dim not in (64, 128):
@@ -38,20 +41,48 @@ class PagedOperator(MLIROperator):
                 raise ValueError(f"{name} must be positive, got {getattr(self, name)}")
         if self.max_pages * self.page_size >= 1 << 31:
             raise ValueError("max_pages * page_size must be below 2^31 tokens")
+        import torch
+
         self._spaces = {}
+        self._captured = {}
         self._wanted = None
+        self._device, self._capturing = torch.cuda.current_device, torch.cuda.is_current_stream_capturing
 
     def workspace_bytes(self) -> int:
         raise NotImplementedError
 
+    def counter_bytes(self) -> int:
+        """Bytes at the start of the workspace that must be zero before its first use."""
+        return 0
+
     def _workspace(self, stream: int):
-        """(address, bytes) of this stream's workspace."""
-        ws = self._spaces.get(stream)
+        """(address, bytes) of the workspace of this stream, or of the graph that it captures."""
+        if self._capturing():
+            return self._graph_workspace(stream)
+        if self._captured:  # the graph keeps the memory, and sets it up again in each replay
+            self._captured = {}
+        key = self._device(), stream
+        ws = self._spaces.get(key)
         if ws is None:
             import torch
 
             t = torch.zeros(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
-            ws = self._spaces[stream] = (t.data_ptr(), t.numel(), t)
+            ws = self._spaces[key] = (t.data_ptr(), t.numel(), t)
+        return ws[0], ws[1]
+
+    def _graph_workspace(self, stream: int):
+        import torch
+
+        capture = ctypes.c_uint64()
+        _lib.call("iron_capture_id", stream, ctypes.byref(capture))
+        key = capture.value, stream
+        ws = self._captured.get(key)
+        if ws is None:
+            t = torch.empty(max(16, self.workspace_bytes()), dtype=torch.uint8, device="cuda")
+            if self.counter_bytes():
+                t[: self.counter_bytes()].zero_()  # part of the graph
+            ws = (t.data_ptr(), t.numel(), t)
+            self._captured = {k: w for k, w in self._captured.items() if k[0] == key[0]} | {key: ws}
         return ws[0], ws[1]
 
     def prepare(self):
@@ -74,6 +105,11 @@ class PagedOperator(MLIROperator):
                                             view and t.shape == view and t.stride(-1) == 1):
                 self._refuse_buffers(bufs)
 
+    def _refuse_device(self, bufs, device):
+        for i, t in enumerate(bufs):
+            if address(t) and t.get_device() != device:
+                raise ValueError(f"buffer {i} of {type(self).__name__} is on {t.device}, the current device is {device}")
+
     def _refuse_buffers(self, bufs):
         """Raises for what is wrong with the buffers."""
         me = type(self).__name__
@@ -93,13 +129,17 @@ class PagedOperator(MLIROperator):
 
         _lib.load()
         written = [i for i, s in enumerate(self.get_arg_spec()) if s.direction != "in"]
-        check, launch, device = self._check_buffers, self._launch, torch.cuda.current_device
+        check, refuse, launch, device = self._check_buffers, self._refuse_device, self._launch, torch.cuda.current_device
+        several = torch.cuda.device_count() > 1
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
         def call(*bufs):
             tensors = [getattr(b, "device_tensor", b) for b in bufs]
             check(tensors)
-            launch(*tensors, stream=raw(device()))
+            at = device()
+            if several:
+                refuse(tensors, at)
+            launch(*tensors, stream=raw(at))
             for i in written:
                 if bufs[i] is not tensors[i]:
                     bufs[i].mark_device_written()

@@ -40,3 +40,12 @@ extern "C" const char *iron_strerror(int status) {
 extern "C" int iron_last_cuda_error(void) { return iron::g_last_cuda_error; }
 
 extern "C" int iron_abi_version(void) { return (1 << 16) | 1; }
+
+extern "C" int iron_capture_id(void *stream, unsigned long long *id) {
+  if (!id) return IRON_ERR_NULL;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  const int st = iron::call_status(cudaStreamGetCaptureInfo_v2(static_cast<cudaStream_t>(stream), &status, &capture));
+  *id = st == IRON_OK && status == cudaStreamCaptureStatusActive ? capture : 0;
+  return st;
+}

@@ -362,8 +362,16 @@ static size_t tree_counters(int B, int N, int Hq, int Hkv, int head_dim) {
   return ((2 * static_cast<size_t>(tree_pieces(head_dim, 16)) + units) * sizeof(unsigned) + 15) / 16 * 16;
 }
 
+static bool no_tree(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
+  return batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128);
+}
+
+extern "C" size_t iron_tree_attn_counter_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
+  return no_tree(batch, num_nodes, num_heads, kv_heads, head_dim) ? 0 : tree_counters(batch, num_nodes, num_heads, kv_heads, head_dim);
+}
+
 extern "C" size_t iron_tree_attn_workspace_bytes(int batch, int num_nodes, int num_heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || num_nodes <= 0 || num_heads <= 0 || kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (no_tree(batch, num_nodes, num_heads, kv_heads, head_dim)) return 0;
   // the counters, then the partials of any form
   const size_t f16 = static_cast<size_t>(tree_pieces(head_dim, 16)) * 2 * 16 * (2 + head_dim) * sizeof(float);
   const size_t f32 = static_cast<size_t>(tree_pieces(head_dim, 32)) * 2 * 32 * (2 + head_dim) * sizeof(float);

@@ -72,6 +72,10 @@ class TreeAttention(PagedOperator):
         return _lib.load().iron_tree_attn_workspace_bytes(self.batch, self.num_nodes, self.num_heads,
                                                           self.num_kv_heads, self.head_dim)
 
+    def counter_bytes(self) -> int:
+        return _lib.load().iron_tree_attn_counter_bytes(self.batch, self.num_nodes, self.num_heads, self.num_kv_heads,
+                                                        self.head_dim)
+
     def _launch(self, q, k_new, v_new, k_pages, v_pages, page_table, lens, parents, out, *, stream, flags=0):
         p = address
         new = (self.batch, self.num_nodes, self.num_kv_heads, self.head_dim)
