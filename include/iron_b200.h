@@ -453,7 +453,7 @@ typedef struct {
  * slot is refused whole (lens_out = lens, nothing written) if the pages run out before it,
  * if its table row is too short, or if it would write a page that another row holds too;
  * *status gets the number of refused slots. With codes, pages that become full get their
- * summary. slots <= 2048. `workspace` >= iron_page_append_workspace_bytes. */
+ * summary, and kv_heads * head_dim is at most 51200. slots <= 2048. `workspace` >= iron_page_append_workspace_bytes. */
 size_t iron_page_append_workspace_bytes(int slots, int num_pages);
 int iron_page_append(const iron_page_pool *pool, const uint16_t *k_new, const uint16_t *v_new,
                      const int32_t *index, int num_new, int32_t *lens_out, int32_t *status,

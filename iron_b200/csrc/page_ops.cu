@@ -610,19 +610,20 @@ extern "C" int iron_page_append(const iron_page_pool *c, const uint16_t *k_new, 
   a.P = c->num_pages;
   a.M = c->max_pages;
   a.layer_stride = static_cast<int64_t>(a.P) * a.Hkv * a.page * a.D;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int st = launch(append_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, a);
-  if (st != IRON_OK) return st;
   const int touched = min((num_new + a.page - 2) / a.page + 1, a.M);
   const int vpr = a.Hkv * a.D / 8, width = vpr < kAppendThreads ? vpr : kAppendThreads;
   const int groups = kAppendThreads / width < 64 ? kAppendThreads / width : 64;
   const size_t smem = a.codes ? static_cast<size_t>(groups) * 2 * a.Hkv * a.D * sizeof(uint16_t) : 0;
+  // nothing may be refused once the plan runs: it takes pages and moves the lengths
   if (smem > 200 * 1024) return IRON_ERR_UNSUPPORTED;
   auto kern = a.codes ? append_write_kernel<true> : append_write_kernel<false>;
   if (smem > 48 * 1024) {
     const int e = call_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     if (e != IRON_OK) return e;
   }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int st = launch(append_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, true, a);
+  if (st != IRON_OK) return st;
   return launch(kern, dim3(touched, a.S, 2 * a.layers), dim3(kAppendThreads), smem, s, true, a);
 }
 

@@ -77,6 +77,8 @@ class PageAppend(_PoolOperator):
     def __post_init__(self):
         if self.num_new < 1:
             raise ValueError(f"num_new must be positive, got {self.num_new}")
+        if self.summaries and self.num_kv_heads * self.head_dim > 51200:
+            raise ValueError("with summaries num_kv_heads * head_dim must be at most 51200")
         super().__post_init__()
 
     def get_arg_spec(self):
