@@ -25,7 +25,7 @@ import torch
 
 from ... import _lib
 from ...operators import PageAppend, PagedKVCache, PageSelectAttention, TreeAttention
-from .decode import LlamaDecodeEngine
+from .decode import LlamaDecodeEngine, rope_table
 
 
 def lookup_draft(text, nodes: int):
@@ -66,7 +66,9 @@ class PagedDecoder:
     def __init__(self, engine: LlamaDecodeEngine, slots: int, nodes: int, num_pages: int, page_size: int = 64,
                  max_pages: int | None = None, top_pages: int | None = None):
         """nodes: drafted tokens per slot and pass, the root included (slots * nodes <= 64, the
-        int4 GEMV's vectors); top_pages: pages that decode_selected reads per kv head."""
+        int4 GEMV's vectors); max_pages: pages of a slot (those of the engine's max_seq tokens
+        unless given; a slot may grow past max_seq, only a prompt may not); top_pages: pages that
+        decode_selected reads per kv head."""
         if not 1 <= slots * nodes <= 64:
             raise ValueError(f"slots * nodes must be 1 to 64, got {slots} * {nodes}")
         self.engine, self.s, self.slots, self.nodes = engine, engine.s, slots, nodes
@@ -83,6 +85,8 @@ class PagedDecoder:
         self._layer_append = PageAppend(slots=slots, num_layers=1, num_new=1, summaries=True, **sizes).get_callable()
         self._row_append, self._sizes = {}, sizes
         dev, bf = engine.dev, dict(dtype=torch.bfloat16, device=engine.dev)
+        # angles of every position that a slot and the drafts behind it can have
+        self._lut = rope_table(s.head_dim, max_pages * page_size + nodes, s.rope_base, dev)
         R = slots * nodes
         self._x, self._xn, self._h = (torch.zeros(R, s.emb_dim, **bf) for _ in range(3))
         self._qkv, self._rot = (torch.zeros(R, s.n_heads + 2 * s.n_kv_groups, s.head_dim, **bf) for _ in range(2))
@@ -109,7 +113,7 @@ class PagedDecoder:
             call("iron_rmsnorm", p(x), None, None, p(lay["n1"]), p(xn), R, E, s.eps, 0, st)
             call("iron_gemv_int4g32", p(lay["qkv"].packed), p(xn), p(qkv), s.qkv_dim, E, R, None, 0, st)
             # every head of a token is rotated by the token's angle; v is taken from qkv
-            call("iron_rope", p(qkv), None, p(e.lut), p(rot), R * (Hq + 2 * G), D, R, p(positions), 0, 0, st)
+            call("iron_rope", p(qkv), None, p(self._lut), p(rot), R * (Hq + 2 * G), D, R, p(positions), 0, 0, st)
             attend(li, rot[:, :Hq], rot[:, Hq : Hq + G], qkv[:, Hq + G :], attn)
             call("iron_gemv_int4g32", p(lay["o"].packed), p(attn), p(h), E, Hq * D, R, p(x), 0, st)
             call("iron_rmsnorm", p(h), None, None, p(lay["n2"]), p(xn), R, E, s.eps, 0, st)
@@ -151,7 +155,7 @@ class PagedDecoder:
         for _ in range(N):  # a node's depth: how often its parent has one
             depth += up >= 0
             up = torch.where(up >= 0, torch.gather(parents, 1, up.clamp(0, N - 1).long()), up)
-        positions = (c.lens[:, None] + depth).clamp(max=self.engine.L - 1).reshape(-1).contiguous()
+        positions = (c.lens[:, None] + depth).reshape(-1).contiguous()
 
         def attend(li, q, k, v, out):
             self._k[li].copy_(k.view(B, N, G, D))
@@ -216,7 +220,7 @@ class PagedDecoder:
         c, B = self.cache, self.slots
         index = torch.zeros(B, 1, **self._ints)
         after = c.lens + 1
-        positions = c.lens.clamp(max=self.engine.L - 1)
+        positions = c.lens.clone()
         last = self.s.n_layers - 1
         refused = torch.zeros_like(self._status)
 

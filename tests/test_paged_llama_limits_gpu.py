@@ -1,0 +1,61 @@
+"""The paged decoder at the ends of its room: sequences past the engine's own cache, outputs
+that exactly fill the table, refusals."""
+
+import pytest
+import torch
+
+from test_paged_llama_gpu import TOL, agree, plain_logits, prompt
+
+pytestmark = pytest.mark.gpu
+
+from iron_b200.applications.llama_3_2_1b.decode import LlamaDecodeEngine, LlamaShape
+from iron_b200.applications.llama_3_2_1b.paged import PagedDecoder
+
+SHAPE = dict(n_layers=2, vocab_size=4096)
+
+
+@pytest.fixture(scope="module")
+def engine():
+    return LlamaDecodeEngine(LlamaShape(**SHAPE), batch=1, max_seq=310, seed=3, fuse_norm="none")
+
+
+@pytest.fixture(scope="module")
+def longer():
+    """The same weights with room for more tokens."""
+    return LlamaDecodeEngine(LlamaShape(**SHAPE), batch=1, max_seq=480, seed=3, fuse_norm="none")
+
+
+def same_keys(decoder, engine, first, last):
+    """The cached keys of tokens first .. last - 1 (of both layers) are those of the plain decode."""
+    c = decoder.cache
+    ids = c.page_table[0, : -(-last // 16)].long()
+    got = c.k[:, ids].transpose(1, 2).flatten(2, 3)[:, :, first:last].float()
+    ref = engine.kc[:, 0, :, first:last].float()
+    assert float(((got - ref).norm(dim=-1) / ref.norm(dim=-1)).max()) < TOL
+
+
+def test_drafts_past_the_engines_tokens_are_rotated_by_their_own_angles(engine, longer):
+    d = PagedDecoder(engine, slots=1, nodes=8, num_pages=40, page_size=16, max_pages=30)
+    text = prompt(307, 1)
+    d.prefill(text, 0)
+    new = prompt(24, 2)
+    ref = plain_logits(longer, text + new, len(text))
+    parents = torch.tensor([list(range(-1, 7))], dtype=torch.int32, device="cuda")
+    for at in range(0, 24, 8):  # positions 307 to 330
+        d.verify(torch.tensor([new[at : at + 8]], dtype=torch.int32, device="cuda"), parents)
+        agree(d.logits.float(), ref[at : at + 8])
+        d.accept([list(range(8))])
+    d.cache.check()
+    same_keys(d, longer, len(text), len(text) + len(new) - 1)
+
+
+def test_selected_decode_past_the_engines_tokens(engine, longer):
+    d = PagedDecoder(engine, slots=1, nodes=1, num_pages=40, page_size=16, max_pages=30)
+    text, new = prompt(305, 3), prompt(12, 4)
+    d.prefill(text, 0)
+    rows = []
+    for t in new:
+        d.decode_selected(torch.tensor([t], dtype=torch.int32, device="cuda"))
+        rows.append(d.logits[0].float().clone())
+    agree(torch.stack(rows), plain_logits(longer, text + new, len(text)))
+    same_keys(d, longer, len(text), len(text) + len(new) - 1)
