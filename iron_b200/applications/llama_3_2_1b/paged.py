@@ -178,7 +178,8 @@ class PagedDecoder:
 
     def generate(self, prompts, max_new: int, stop: int | None = None):
         """Greedy continuations (lists of max_new tokens, or up to `stop`) of at most `slots`
-        prompts, decoded speculatively. Finished slots are freed."""
+        prompts, decoded speculatively. Finished slots are freed. A prompt and its continuation need
+        room for all their tokens but the last."""
         if not 1 <= len(prompts) <= self.slots:
             raise ValueError(f"generate takes 1 to {self.slots} prompts, got {len(prompts)}")
         dev, N = self.engine.dev, self.nodes
@@ -202,16 +203,21 @@ class PagedDecoder:
             predicted = self.verify(tokens, parents).tolist()
             TreeAttention.check()
             self.passes += 1
-            paths = [[]] * self.slots
-            for i, t in enumerate(texts):
+            paths, more = [[] for _ in range(self.slots)], [[] for _ in texts]
+            for i, (t, p) in enumerate(zip(texts, prompts)):
                 if done[i]:
                     continue
-                paths[i] = accepted_path(*drafts[i], predicted[i])
-                new = [predicted[i][n] for n in paths[i]]
-                if stop in new:
-                    new = new[: new.index(stop) + 1]
+                path = accepted_path(*drafts[i], predicted[i])
+                left = max_new - (len(t) - len(p))
+                more[i] = [predicted[i][n] for n in path][:left]
+                if stop in more[i]:
+                    more[i] = more[i][: more[i].index(stop) + 1]
+                if len(more[i]) < left and more[i][-1] != stop:
+                    paths[i] = path  # the slot goes on: the next pass reads these rows
+            if any(paths):
+                self.accept(paths)
+            for t, new in zip(texts, more):
                 t.extend(new)
-            self.accept(paths)
 
     # -- long contexts -----------------------------------------------------------------------------
     def decode_selected(self, tokens):

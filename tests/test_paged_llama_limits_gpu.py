@@ -59,3 +59,30 @@ def test_selected_decode_past_the_engines_tokens(engine, longer):
         rows.append(d.logits[0].float().clone())
     agree(torch.stack(rows), plain_logits(longer, text + new, len(text)))
     same_keys(d, longer, len(text), len(text) + len(new) - 1)
+
+
+def drafts_from(monkeypatch, known):
+    """generate drafts what is known of the text as a chain (all of it is accepted)."""
+
+    def draft(text, nodes):
+        chain = [text[-1]] + known[len(text) : len(text) + nodes - 1]
+        pad = nodes - len(chain)
+        return chain + [0] * pad, list(range(-1, len(chain) - 1)) + [-2] * pad
+
+    monkeypatch.setattr("iron_b200.applications.llama_3_2_1b.paged.lookup_draft", draft)
+
+
+@pytest.mark.parametrize("max_new", [2, 9, 20, 22])
+def test_output_that_just_fits_does_not_depend_on_lucky_drafts(engine, monkeypatch, max_new):
+    """The last pass may accept more than is wanted: those rows need no room."""
+    text = prompt(300, 5)
+    d = PagedDecoder(engine, slots=1, nodes=8, num_pages=40, page_size=16, max_pages=30)
+    out = d.generate([text], 40)[0]
+    known = text + out
+    small = PagedDecoder(engine, slots=1, nodes=8, num_pages=20, page_size=16, max_pages=20)  # 320 tokens
+    drafts_from(monkeypatch, known)
+    assert small.generate([text], max_new)[0] == out[:max_new]
+    assert small.passes <= -(-max_new // 8) + 1  # the drafts were accepted
+    small.cache.check()
+    assert not bool(small.cache.refs.any())
+    assert small.generate([text], max_new, stop=out[1])[0] == out[: min(max_new, out.index(out[1]) + 1)]
