@@ -179,9 +179,10 @@ class PagedDecoder:
     def generate(self, prompts, max_new: int, stop: int | None = None):
         """Greedy continuations (lists of max_new tokens, or up to `stop`) of at most `slots`
         prompts, decoded speculatively. Finished slots are freed. A prompt and its continuation need
-        room for all their tokens but the last."""
+        room for all their tokens but the last; RuntimeError if the cache refuses a slot."""
         if not 1 <= len(prompts) <= self.slots:
             raise ValueError(f"generate takes 1 to {self.slots} prompts, got {len(prompts)}")
+        self.cache.check()  # a refusal from before is not this one's
         dev, N = self.engine.dev, self.nodes
         self.cache.free(range(self.slots))
         texts = [list(p) for p in prompts]
@@ -195,7 +196,6 @@ class PagedDecoder:
                     done[i] = True
                     self.cache.free([i])
             if all(done):
-                self.cache.check()
                 return [t[len(p) : len(p) + max_new] for t, p in zip(texts, prompts)]
             drafts = [lookup_draft(t, N) if not d else ([0] * N, [-2] * N) for t, d in zip(texts, done)]
             drafts += [([0] * N, [-2] * N)] * (self.slots - len(texts))
@@ -216,6 +216,7 @@ class PagedDecoder:
                     paths[i] = path  # the slot goes on: the next pass reads these rows
             if any(paths):
                 self.accept(paths)
+                self.cache.check()
             for t, new in zip(texts, more):
                 t.extend(new)
 

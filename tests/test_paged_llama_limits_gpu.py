@@ -86,3 +86,26 @@ def test_output_that_just_fits_does_not_depend_on_lucky_drafts(engine, monkeypat
     small.cache.check()
     assert not bool(small.cache.refs.any())
     assert small.generate([text], max_new, stop=out[1])[0] == out[: min(max_new, out.index(out[1]) + 1)]
+
+
+def test_a_refused_slot_ends_generate_at_once(engine, monkeypatch):
+    """Pages run out in the middle: the text must not go on over a cache that lacks its rows."""
+    text = prompt(40, 6)
+    d = PagedDecoder(engine, slots=1, nodes=8, num_pages=3, page_size=16)
+    drafts_from(monkeypatch, [])
+    with pytest.raises(RuntimeError, match="refused"):
+        d.generate([text], 60)
+    assert d.passes == 9  # 8 tokens fit the third page
+    assert len(d.generate([text], 9)[0]) == 9  # and the decoder is usable
+
+
+def test_a_refusal_from_before_is_raised_before_generate_starts(engine):
+    d = PagedDecoder(engine, slots=1, nodes=8, num_pages=2, page_size=16)
+    d.prefill(prompt(30, 7), 0)
+    d.verify(*(torch.zeros(1, 8, dtype=torch.int32, device="cuda") - i for i in (0, 1)))
+    d.accept([list(range(8))])
+    d.passes = -1
+    with pytest.raises(RuntimeError, match="refused"):
+        d.generate([prompt(10, 8)], 2)
+    assert d.passes == -1
+    assert len(d.generate([prompt(10, 8)], 2)[0]) == 2
