@@ -223,7 +223,8 @@ class PagedDecoder:
     # -- long contexts -----------------------------------------------------------------------------
     def decode_selected(self, tokens):
         """One token per slot (int32 [slots], device), read through the selected pages: appends
-        its keys and values and returns the predictions, int32 [slots]. Every slot takes part."""
+        its keys and values and returns the predictions, int32 [slots]. Every slot takes part: if
+        the cache refuses one, RuntimeError, and all keep their lengths."""
         c, B = self.cache, self.slots
         index = torch.zeros(B, 1, **self._ints)
         after = c.lens + 1
@@ -244,5 +245,6 @@ class PagedDecoder:
 
         out = self._forward(tokens, positions, attend)
         if int(refused):
+            c.lens.copy_(positions)  # the others' rows are written again when the step is repeated
             raise RuntimeError("a slot was refused: no free page, a full table row, or a shared page to be written")
         return out

@@ -109,3 +109,18 @@ def test_a_refusal_from_before_is_raised_before_generate_starts(engine):
         d.generate([prompt(10, 8)], 2)
     assert d.passes == -1
     assert len(d.generate([prompt(10, 8)], 2)[0]) == 2
+
+
+def test_a_refused_selected_step_moves_no_slot(engine):
+    d = PagedDecoder(engine, slots=2, nodes=1, num_pages=2, page_size=16)
+    texts = [prompt(16, 9), prompt(5, 10)]
+    for i, t in enumerate(texts):
+        d.prefill(t, i)
+    step = torch.tensor([7, 9], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="refused"):
+        d.decode_selected(step)  # slot 0 needs a third page
+    assert d.cache.lens.tolist() == [16, 5]
+    d.cache.free([0])
+    d.decode_selected(step)
+    assert d.cache.lens.tolist() == [1, 6]
+    agree(d.logits[1:].float(), plain_logits(engine, texts[1] + [9], 5))
