@@ -128,8 +128,12 @@ class PagedDecoder:
     # -- cache ---------------------------------------------------------------------------------
     def prefill(self, tokens, slot: int):
         """Runs a prompt through the engine and puts its keys and values into the slot's pages
-        (the slot must be empty). Returns the model's next token."""
+        (ValueError if the slot is not empty). Returns the model's next token."""
         e, c, n = self.engine, self.cache, len(tokens)
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot must be 0 to {self.slots - 1}, got {slot}")
+        if int(c.lens[slot]):
+            raise ValueError(f"slot {slot} holds {int(c.lens[slot])} tokens: free it first")
         e.prefill(tokens, 0)
         if n not in self._row_append:
             self._row_append[n] = PageAppend(slots=1, num_layers=self.s.n_layers, num_new=n, summaries=True,

@@ -124,3 +124,18 @@ def test_a_refused_selected_step_moves_no_slot(engine):
     d.decode_selected(step)
     assert d.cache.lens.tolist() == [1, 6]
     agree(d.logits[1:].float(), plain_logits(engine, texts[1] + [9], 5))
+
+
+def test_a_prompt_needs_an_empty_slot(engine):
+    """Its keys are rotated for positions 0, 1, ...; behind other tokens they would be wrong."""
+    d = PagedDecoder(engine, slots=2, nodes=1, num_pages=8, page_size=16)
+    d.prefill(prompt(20, 11), 1)
+    with pytest.raises(ValueError, match="slot 1 holds 20 tokens"):
+        d.prefill(prompt(5, 12), 1)
+    for slot in (-1, 2):
+        with pytest.raises(ValueError, match="slot must be"):
+            d.prefill(prompt(5, 12), slot)
+    assert d.cache.lens.tolist() == [0, 20]
+    d.cache.free([1])
+    d.prefill(prompt(5, 12), 1)
+    assert d.cache.lens.tolist() == [0, 5]
