@@ -83,7 +83,9 @@ class PagedDecoder:
         self._select = PageSelectAttention(batch=slots, top_pages=top, **sizes).get_callable()
         sizes.pop("num_heads")
         self._layer_append = PageAppend(slots=slots, num_layers=1, num_new=1, summaries=True, **sizes).get_callable()
-        self._row_append, self._sizes = {}, sizes
+        # prompts: one operator per length, on shared workspaces
+        self._row_append, self._row_sizes = {}, dict(slots=1, num_layers=s.n_layers, summaries=True, **sizes)
+        self._first_row = PageAppend(**self._row_sizes)
         dev, bf = engine.dev, dict(dtype=torch.bfloat16, device=engine.dev)
         # angles of every position that a slot and the drafts behind it can have
         self._lut = rope_table(s.head_dim, max_pages * page_size + nodes, s.rope_base, dev)
@@ -136,8 +138,8 @@ class PagedDecoder:
             raise ValueError(f"slot {slot} holds {int(c.lens[slot])} tokens: free it first")
         e.prefill(tokens, 0)
         if n not in self._row_append:
-            self._row_append[n] = PageAppend(slots=1, num_layers=self.s.n_layers, num_new=n, summaries=True,
-                                             **self._sizes).get_callable()
+            op = PageAppend(num_new=n, **self._row_sizes)
+            self._row_append[n] = op.share_workspaces(self._first_row).get_callable()
         k, v = (x[:, 0, :, :n].transpose(1, 2).contiguous() for x in (e.kc, e.vc))
         row = slice(slot, slot + 1)
         index = torch.arange(n, **self._ints)

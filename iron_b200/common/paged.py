@@ -51,6 +51,12 @@ class PagedOperator(MLIROperator):
     def workspace_bytes(self) -> int:
         raise NotImplementedError
 
+    def share_workspaces(self, other: "PagedOperator"):
+        """Calls of this operator use the workspaces of `other`, whose size must do for both, and
+        must not overlap its calls on the same stream. Returns self."""
+        self._spaces = other._spaces
+        return self
+
     def counter_bytes(self) -> int:
         """Bytes at the start of the workspace that must be zero before its first use."""
         return 0

@@ -169,7 +169,8 @@ class PagedKVCache:
                            page_size=page_size, num_pages=num_pages, max_pages=max_pages)
         self._fork = PageFork(**self._sizes)
         self._compact = PageCompact(**self._sizes, summaries=summaries)
-        self._append = {}
+        # one operator per number of new rows; their workspaces are of one size, and shared
+        self._append, self._first_append = {}, PageAppend(**self._sizes, summaries=summaries)
         self.summaries = summaries
         dev = torch.device("cuda", torch.cuda.current_device())
         pool = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
@@ -192,7 +193,8 @@ class PagedKVCache:
         """k_new, v_new [num_layers, slots, n, num_kv_heads, head_dim], index int32 [slots, n]."""
         n = index.shape[1]
         if n not in self._append:
-            self._append[n] = PageAppend(**self._sizes, num_new=n, summaries=self.summaries).get_callable()
+            op = PageAppend(**self._sizes, num_new=n, summaries=self.summaries)
+            self._append[n] = op.share_workspaces(self._first_append).get_callable()
         self._append[n](k_new, v_new, index, self.k, self.v, self.page_table, self.lens, self.refs, self.lens,
                         self._status, *self._summary())
         self._refused += self._status
