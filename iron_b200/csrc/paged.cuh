@@ -55,6 +55,18 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], const void *p) {
                : "memory");
 }
 
+// Two p >= 0 as two bf16 parts each: hi is p cut off after 8 bits, lo = kSplit p - hi, rounded
+// (minus0 and minus1 are the -hi). Both parts are positive where p is, so that a value of +-inf
+// times them stays one: 0 * inf, or infinities of both signs, would be NaN.
+constexpr float kSplit = 1.f + 1.f / 1048576.f;
+__device__ __forceinline__ uint32_t split_hi(float p0, float p1, float &minus0, float &minus1) {
+  uint32_t hi;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(p1), "f"(p0));
+  minus0 = __uint_as_float(hi << 16 | 0x80000000u);
+  minus1 = __uint_as_float((hi & 0xffff0000u) | 0x80000000u);
+  return hi;
+}
+
 // A stage: 16 rows of K, then 16 rows of V.
 template <int D>
 struct Stage {
@@ -159,8 +171,9 @@ struct WarpAttn {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float p0 = s[i >> 1][2 * (i & 1)], p1 = s[i >> 1][2 * (i & 1) + 1];
-      hi[i] = pack_bf16x2(p0, p1);
-      lo[i] = pack_bf16x2(p0 - bf16_lo(hi[i]), p1 - bf16_hi(hi[i]));
+      float m0, m1;
+      hi[i] = split_hi(p0, p1, m0, m1);
+      lo[i] = pack_bf16x2(fmaf(p0, kSplit, m0), fmaf(p1, kSplit, m1));
     }
 #pragma unroll
     for (int jp = 0; jp < D / 16; ++jp) {

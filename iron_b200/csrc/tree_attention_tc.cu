@@ -605,7 +605,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             ref = 0.f;
             by = 1.f;
           }
-          const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), minus = pack2(-1.f, -1.f);
+          const uint64_t by2 = pack2(by, by), ref2 = pack2(-ref, -ref), split = pack2(kSplit, kSplit);
           uint64_t sum[4] = {0, 0, 0, 0};
           uint32_t hi[32], lo[32];
 #pragma unroll
@@ -616,8 +616,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const TreeArgs a) {
             p1 = ex2_approx(p1);
             const uint64_t p = pack2(p0, p1);
             sum[q & 3] = add2(sum[q & 3], p);
-            hi[q] = pack_bf16x2(p0, p1);
-            unpack2(fma2(pack2(bf16_lo(hi[q]), bf16_hi(hi[q])), minus, p), p0, p1);
+            float m0, m1;
+            hi[q] = split_hi(p0, p1, m0, m1);
+            unpack2(fma2(p, split, pack2(m0, m1)), p0, p1);
             lo[q] = pack_bf16x2(p0, p1);
           }
           // the P V before has read P (only one may be under way)
