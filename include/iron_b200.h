@@ -426,7 +426,7 @@ int iron_attn_prefill(const uint16_t *q, const uint16_t *k, const uint16_t *v, u
  *            -1 for no page;
  *   lens     int32 [slots]: tokens of each slot;
  *   refs     int32 [num_pages]: how many table rows hold the page (0: free).
- * head_dim 64 or 128; page_size 16, 32, 64 or 128; page * max_pages < 2^31; pools and
+ * head_dim 64 or 128; page_size 16, 32, 64 or 128; page * max_pages <= 2^31 - 128; pools and
  * codes 16-byte aligned. Table entries outside [0, num_pages) are never followed.
  * Tables, lengths and counts are read on the device, by several CTAs each for itself: nothing
  * may write them while a call runs (a writer on another stream needs an event in between).
@@ -486,7 +486,8 @@ int iron_page_compact(const iron_page_pool *pool, int32_t *page_table_out, int32
  * softmax; zeros for an unused node. What the path does not hold has no effect, whatever
  * its values. q, out bf16 [batch, num_nodes, Hq, D], k_new, v_new bf16 [batch, num_nodes,
  * kv_heads, D] with element strides {batch, node, head} (3 int64 each, multiples of 8; kv
- * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024.
+ * strides for both k_new and v_new). num_nodes <= 128, Hq / kv_heads <= 16, batch <= 1024,
+ * batch * (page * max_pages / 64 + 5) < 2^31.
  * `workspace` >= iron_tree_attn_workspace_bytes holds counters, in its first
  * iron_tree_attn_counter_bytes, and the partials of what is split. The counters must be zero
  * before the first use; calls leave them zero (one workspace may serve calls of the same sizes

@@ -39,8 +39,8 @@ class PagedOperator(MLIROperator):
         for name in ("num_pages", "max_pages", "num_kv_heads"):
             if getattr(self, name) < 1:
                 raise ValueError(f"{name} must be positive, got {getattr(self, name)}")
-        if self.max_pages * self.page_size >= 1 << 31:
-            raise ValueError("max_pages * page_size must be below 2^31 tokens")
+        if self.max_pages * self.page_size > (1 << 31) - 128:
+            raise ValueError("max_pages * page_size must be at most 2^31 - 128 tokens")
         import torch
 
         self._spaces = {}

@@ -17,7 +17,8 @@ inline int pool_geometry_check(const iron_page_pool *c) {
   if (c->head_dim != 64 && c->head_dim != 128) return IRON_ERR_UNSUPPORTED;
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
     return IRON_ERR_UNSUPPORTED;
-  if (static_cast<int64_t>(c->max_pages) * c->page_size > 0x7fffffff) return IRON_ERR_SHAPE;
+  // a length rounded up to a whole tile (of 128 tokens at most) stays an int
+  if (static_cast<int64_t>(c->max_pages) * c->page_size > 0x7fffffff - 127) return IRON_ERR_SHAPE;
   if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->codes)) return IRON_ERR_ALIGN;
   if ((c->codes != nullptr) != (c->scales != nullptr)) return IRON_ERR_ARG;
   return IRON_OK;

@@ -451,6 +451,9 @@ extern "C" int iron_tree_attn(const iron_page_pool *c, const uint16_t *q, const 
   a.N = num_nodes;
   a.Hq = num_heads;
   a.Hkv = c->kv_heads;
+  // the tiles (and unit costs) of all sequences are counted in ints
+  const int64_t longest = static_cast<int64_t>(c->max_pages) * c->page_size;
+  if (c->slots * ((longest + kTTile - 1) / kTTile + kTMaxNodes / kTTile + 3) > 0x7fffffff) return IRON_ERR_SHAPE;
   const int64_t tiles = full_tiles(c, num_nodes * g);
   const int unit = unit_rows(num_nodes * g, tiles, c->head_dim);
   a.groups = (num_nodes * g + unit - 1) / unit;

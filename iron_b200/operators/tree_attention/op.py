@@ -57,6 +57,8 @@ class TreeAttention(PagedOperator):
         if self.num_kv_heads < 1 or self.num_heads % self.num_kv_heads or not 1 <= self.num_heads // self.num_kv_heads <= 16:
             raise ValueError("num_heads must be a multiple of num_kv_heads (group <= 16)")
         self._check_geometry()
+        if self.batch * (-(-self.max_pages * self.page_size // 64) + 5) >= 1 << 31:
+            raise ValueError("batch * (max_pages * page_size / 64 + 5) must be below 2^31")
         PagedOperator.__init__(self, context=self.context)
 
     def get_arg_spec(self):
