@@ -86,7 +86,8 @@ __device__ __forceinline__ void query_weights(const float (&x)[16], int g, int16
   __syncthreads();
 }
 
-// An fp32 score as an unsigned key of the same order.
+// An fp32 score as an unsigned key of the same order (-0 would come before 0: the caller adds 0,
+// which makes 0 of it).
 __device__ __forceinline__ uint32_t score_key(float s) {
   const uint32_t u = __float_as_uint(s);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kSThreads, kAttend ? SelectCfg<D>::kCtasPerSm 
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lanepart == 0 && i < hi)
-          keys[i] = score_key(fminf(fmaxf(__fmul_rn(__int2float_rn(sum), scale[u]), -FLT_MAX), FLT_MAX));
+          keys[i] = score_key(fminf(fmaxf(__fmul_rn(__int2float_rn(sum), scale[u]) + 0.f, -FLT_MAX), FLT_MAX));
       }
     }
     // ---- 2. all keys here, then the pages to keep: the last page, the first one (top > 1)
