@@ -165,7 +165,8 @@ _stride_arrays: dict = {}
 
 def stride_array(t, shape):
     """Element strides of the leading dimensions of `t` seen as `shape`, as an int64 array for
-    the C entry points (made once per set of strides, so equal strides give the same array)."""
+    the C entry points (made once per set of strides, so equal strides give the same array). A
+    dimension of one element has stride 0: no address depends on what the tensor says there."""
     full = t.stride()
     if t.shape != shape:
         full, step = [1], 1
@@ -173,7 +174,9 @@ def stride_array(t, shape):
             step *= n
             full.append(step)
         full = tuple(reversed(full))
-    a = _stride_arrays.get(full)
+    a = _stride_arrays.get((full, shape))
     if a is None:
-        a = _stride_arrays[full] = (ctypes.c_int64 * (len(full) - 1))(*full[:-1])
+        seen = tuple(0 if n == 1 else s for n, s in zip(shape[:-1], full))
+        a = _stride_arrays.setdefault(seen, (ctypes.c_int64 * len(seen))(*seen))
+        _stride_arrays[full, shape] = a
     return a
