@@ -28,3 +28,16 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def no_wait_runs_out(request):
+    """After every GPU test of the paged operators: no bounded wait of the tree attention ran out."""
+    yield
+    if "gpu" in request.keywords and request.module.__name__.startswith(("test_tree", "test_page")):
+        import torch
+
+        if torch.cuda.is_available():
+            from iron_b200 import _lib
+
+            assert _lib.load().iron_tree_attn_status(1) == 0, "a wait of the tree attention timed out"
