@@ -5,8 +5,9 @@
 // refs int32 [P] counts the table rows that hold a page. Every operator is two launches:
 // a plan by one CTA (who gets which page, from block-wide prefix sums over slots and over
 // the pool's reference counts, so the lowest free pages go out in slot order and the
-// result does not depend on any order of execution) and a grid that moves the rows. The
-// only atomics add to integer reference counts, whose sum has no order.
+// result does not depend on any order of execution; fork has more CTAs beside it, which
+// copy the reference counts) and a grid that moves the rows. The only atomics add to integer
+// reference counts, whose sum has no order.
 //
 // Bounds: the data grids by HBM (each moved row is read once and written once, 16 bytes
 // per thread and access, 4 or 8 accesses in flight per thread); the plans by the latency

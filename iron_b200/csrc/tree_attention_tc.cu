@@ -4,8 +4,9 @@
 // to 256 of them, a tile is 128 tokens. One CTA per SM takes an equal share of all units'
 // tiles (tree.cuh). Two streams of 128 rows run staggered, so that one's softmax overlaps
 // the other's MMAs: with more than 128 rows stream s is the unit's rows 128 s ... and both
-// see every tile; with fewer, both hold the same rows and stream s sees every second tile;
-// stream 0 then joins both results, whose rows lie in the same TMEM lanes.
+// see every tile; with fewer, both hold the same rows and stream s sees every second tile
+// (its issuing warp goes through all of them); stream 0 then joins both results, whose rows
+// lie in the same TMEM lanes.
 //
 // Warps: 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns one row: no shuffles), 8
 // and 9 issue the MMAs of stream 0 and 1, 10 loads (TMA, one box per page and 64 columns),
@@ -21,11 +22,11 @@
 // Bounds (B200): per 128 tokens and stream 1024 cycles of ex2 (16 per cycle and SM for 128
 // rows), and on the tensor cores 250 of S and 530 of P V at D = 64, 770 and 960 at D = 128
 // (measured alone: S of 64 columns 48 cycles per MMA, of 128 columns 62; P V 33 and 60).
-// 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 112 us, D = 128 131 (of 107 at D =
-// 64: without the MMAs 100, without ex2 88, without all arithmetic of the softmax 71): no unit is
+// 16 sequences of 4608 tokens, 64 nodes of 4 heads: D = 64 114 us, D = 128 133 (when D = 64 took
+// 107: without the MMAs 100, without ex2 88, without all arithmetic of the softmax 71): no unit is
 // full (issue 40 %, ex2 36 %, tensor 27 %); the 550 instructions of a warp per 64 tokens, with
 // two such warps per scheduler, set the pace. 8 sequences of
-// 32768 tokens, D = 128: 282 us, tensor cores 70 % busy (335 in long runs, at the power
+// 32768 tokens, D = 128: 296 us, tensor cores 68 % busy (347 in long runs, at the power
 // limit). What a tile must not hold (past the length, unused nodes) is masked in S and
 // zeroed in V.
 #include <cuda.h>

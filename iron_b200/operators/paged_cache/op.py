@@ -158,7 +158,9 @@ class PagedKVCache:
     ``append``, ``fork``, ``free`` and ``compact`` change the cache on the current stream
     without waiting for the GPU; ``check`` waits and raises RuntimeError if one of them
     refused a slot. ``layer(i)`` gives the buffers that TreeAttention (k_pages, v_pages) and
-    PageSelectAttention (with codes and scales) read.
+    PageSelectAttention (with codes and scales) read. ``fork`` and ``free`` write a second set of
+    ``page_table``, ``lens`` and ``refs`` and swap it in, so take these from the cache for each
+    call; a captured graph keeps the set that it was captured with.
     """
 
     def __init__(self, slots: int, num_layers: int, num_kv_heads: int, head_dim: int, page_size: int, num_pages: int,
