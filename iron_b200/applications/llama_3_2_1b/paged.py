@@ -87,8 +87,9 @@ class PagedDecoder:
         self._row_append, self._row_sizes = {}, dict(slots=1, num_layers=s.n_layers, summaries=True, **sizes)
         self._first_row = PageAppend(**self._row_sizes)
         dev, bf = engine.dev, dict(dtype=torch.bfloat16, device=engine.dev)
-        # angles of every position that a slot and the drafts behind it can have
-        self._lut = rope_table(s.head_dim, max_pages * page_size + nodes, s.rope_base, dev)
+        # angles of every position that a slot and the drafts behind it can have (a table may be
+        # wider than the pool)
+        self._lut = rope_table(s.head_dim, min(max_pages, num_pages) * page_size + nodes, s.rope_base, dev)
         R = slots * nodes
         self._x, self._xn, self._h = (torch.zeros(R, s.emb_dim, **bf) for _ in range(3))
         self._qkv, self._rot = (torch.zeros(R, s.n_heads + 2 * s.n_kv_groups, s.head_dim, **bf) for _ in range(2))
@@ -127,6 +128,10 @@ class PagedDecoder:
         call("iron_argmax", p(self.logits), p(self._pred), R, s.vocab_size, None, 0, st)
         return self._pred[:R]
 
+    def _in_table(self, positions):
+        """Positions that the operators' own lengths never pass, whatever someone wrote there."""
+        return positions.clamp(0, self._lut.shape[0] - 1)
+
     # -- cache ---------------------------------------------------------------------------------
     def prefill(self, tokens, slot: int):
         """Runs a prompt through the engine and puts its keys and values into the slot's pages
@@ -161,7 +166,7 @@ class PagedDecoder:
         for _ in range(N):  # a node's depth: how often its parent has one
             depth += up >= 0
             up = torch.where(up >= 0, torch.gather(parents, 1, up.clamp(0, N - 1).long()), up)
-        positions = (c.lens[:, None] + depth).reshape(-1).contiguous()
+        positions = self._in_table(c.lens[:, None] + depth).reshape(-1).contiguous()
 
         def attend(li, q, k, v, out):
             self._k[li].copy_(k.view(B, N, G, D))
@@ -234,7 +239,7 @@ class PagedDecoder:
         c, B = self.cache, self.slots
         index = torch.zeros(B, 1, **self._ints)
         after = c.lens + 1
-        positions = c.lens.clone()
+        before, positions = c.lens.clone(), self._in_table(c.lens)
         last = self.s.n_layers - 1
         refused = torch.zeros_like(self._status)
 
@@ -251,6 +256,6 @@ class PagedDecoder:
 
         out = self._forward(tokens, positions, attend)
         if int(refused):
-            c.lens.copy_(positions)  # the others' rows are written again when the step is repeated
+            c.lens.copy_(before)  # the others' rows are written again when the step is repeated
             raise RuntimeError("a slot was refused: no free page, a full table row, or a shared page to be written")
         return out

@@ -139,3 +139,11 @@ def test_a_prompt_needs_an_empty_slot(engine):
     d.cache.free([1])
     d.prefill(prompt(5, 12), 1)
     assert d.cache.lens.tolist() == [0, 5]
+
+
+def test_a_wide_table_takes_no_memory_for_angles(engine):
+    """A slot holds no more tokens than the pool has, however wide its table row is."""
+    d = PagedDecoder(engine, slots=1, nodes=3, num_pages=8, page_size=16, max_pages=100000, top_pages=4)
+    assert d._lut.shape[0] == 8 * 16 + 3
+    text = prompt(120, 13)
+    assert d.generate([text], 9)[0] == PagedDecoder(engine, slots=1, nodes=3, num_pages=8, page_size=16).generate([text], 9)[0]
